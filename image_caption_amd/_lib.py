@@ -17,6 +17,9 @@ PRECISION_FP32, PRECISION_BF16, PRECISION_F32_SPLIT = 0, 1, 2
 CELL_LSTM, CELL_GRU = 0, 1
 MAX_BEAM_WIDTH = 16
 BEAM_STEP_STATIC_MAX_ROWS = 16384
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+MAX_ALTERNATIVES = 32
+MAX_TEACHER_LOGITS = 256
 K_NAMES = ("encode", "feat_proj", "init_state", "attn_query", "attention", "lstm", "fc1",
            "vocab", "beam", "backtrack")
 
@@ -77,7 +80,7 @@ class IcapTWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in TWEIGHT_FIELDS] + [("layers", C.POINTER(IcapTLayer))]
 
 
-_P, _I, _F, _D = C.c_void_p, C.c_int, C.c_float, C.c_double
+_P, _I, _F, _D, _L = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_longlong
 
 # name -> argtypes; every entry point of include/icap.h
 SIGNATURES = {
@@ -103,6 +106,12 @@ SIGNATURES = {
     "icap_beam_step_static_f32": ([_P, _P, _P, _P, _I, _I, _I, _D, _I, _P, _P, _P, _P, _P, _P,
                                    _I, _I, _I, _P], C.c_int),
     "icap_sample_categorical_f32": ([_P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P], C.c_int),
+    "icap_token_log_probs": ([_P, _I, _I, _I, _I, _L, _L, _P, _I, _I] + [_P] * 6, C.c_int),
+    "icap_token_log_probs_grad": ([_P, _I, _I, _I, _I, _L, _L, _P, _I] + [_P] * 5 + [_L, _L, _P], C.c_int),
+    "icap_distill_loss": ([_P, _I, _I, _I, _I, _L, _L, _P, _I, _P, _I, _F, _P, _P, _P, _L, _L, _P], C.c_int),
+    "icap_embedding_scaled": ([_P, _I, _P, _P, _I, _I, _I, _F, _I, _P], C.c_int),
+    "icap_embedding_grad_workspace_bytes": ([_I, _I, _I], C.c_size_t),
+    "icap_embedding_grad": ([_P, _I, _P, _P, _I, _I, _I, _F, _I, _P, C.c_size_t, _P], C.c_int),
     "icap_backtrack": ([_P] * 7 + [_I, _I, _I, _P], C.c_int),
     "icap_packed_weight_bytes": ([_I, _I], C.c_size_t),
     "icap_pack_weight_bf16": ([_P, _P, _I, _I, _I, _I, _I, _P], C.c_int),

@@ -1,0 +1,212 @@
+// A row of logits over the vocabulary, read once: typed loads of 16 bytes and the running
+// soft-max statistics (gfx950 only).  Shared by the operators that score tokens.
+#pragma once
+
+#include "icap_common.h"
+
+namespace icap {
+
+// Row r of a [N,V] view starts at (r / inner) * ld_outer + (r % inner) * ld elements: a matrix
+// (inner >= N), or the first T - 1 positions of a [B,T,V] tensor (inner = T - 1).
+struct RowView {
+  int inner;
+  long long ld, ld_outer;
+  __host__ __device__ size_t at(int r) const {
+    return r < inner ? (size_t)r * (size_t)ld
+                     : (size_t)(r / inner) * (size_t)ld_outer + (size_t)(r % inner) * (size_t)ld;
+  }
+};
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+// A difference to the row maximum is held at this: -inf and the lowest float are at -1e30 all the
+// same a weight of exactly 0, and 0 * -1e30 stays 0 where 0 * -inf would not.
+constexpr float kFarBelow = -1e30f;
+
+#if defined(__HIPCC__)
+
+// Rows start at any element, so the loads are declared with the element's alignment only; the
+// hardware takes global accesses of 16 bytes at any address.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <int DTYPE>
+struct Elem;
+
+template <>
+struct Elem<ICAP_DTYPE_F32> {
+  typedef float type;
+  static constexpr int kVec = 4;
+  __device__ static float up(float v) { return v; }
+  __device__ static float down(float v) { return v; }
+  __device__ static void unpack(u32x4 raw, float (&x)[kVec]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(raw[i]);
+  }
+  __device__ static u32x4 pack(const float (&x)[kVec]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(x[i]);
+    return r;
+  }
+};
+
+template <>
+struct Elem<ICAP_DTYPE_BF16> {
+  typedef __bf16 type;
+  static constexpr int kVec = 8;
+  __device__ static float up(__bf16 v) { return (float)v; }
+  __device__ static __bf16 down(float v) { return (__bf16)v; }
+  __device__ static void unpack(u32x4 raw, float (&x)[kVec]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(raw[i] << 16);
+      x[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+    }
+  }
+  __device__ static u32x4 pack(const float (&x)[kVec]) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bf16x2 two = {(__bf16)x[2 * i], (__bf16)x[2 * i + 1]};
+      r[i] = __builtin_bit_cast(uint32_t, two);
+    }
+    return r;
+  }
+};
+
+template <>
+struct Elem<ICAP_DTYPE_F16> {
+  typedef _Float16 type;
+  static constexpr int kVec = 8;
+  __device__ static float up(_Float16 v) { return (float)v; }
+  __device__ static _Float16 down(float v) { return (_Float16)v; }
+  __device__ static void unpack(u32x4 raw, float (&x)[kVec]) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f16x2 two = __builtin_bit_cast(f16x2, (uint32_t)raw[i]);
+      x[2 * i] = (float)two[0];
+      x[2 * i + 1] = (float)two[1];
+    }
+  }
+  __device__ static u32x4 pack(const float (&x)[kVec]) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f16x2 two = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+      r[i] = __builtin_bit_cast(uint32_t, two);
+    }
+    return r;
+  }
+};
+
+// kVec elements from x + col; columns past the row's end read as `fill`.
+template <int DTYPE>
+__device__ __forceinline__ void load_vec(const typename Elem<DTYPE>::type* x, int col, int V,
+                                         float fill, float (&out)[Elem<DTYPE>::kVec]) {
+  constexpr int kVec = Elem<DTYPE>::kVec;
+  if (col + kVec <= V) {
+    Elem<DTYPE>::unpack(*reinterpret_cast<const u32x4_any*>(x + col), out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) out[i] = col + i < V ? Elem<DTYPE>::up(x[col + i]) : fill;
+  }
+}
+
+template <int DTYPE>
+__device__ __forceinline__ void store_vec(typename Elem<DTYPE>::type* x, int col, int V,
+                                          const float (&v)[Elem<DTYPE>::kVec]) {
+  constexpr int kVec = Elem<DTYPE>::kVec;
+  if (col + kVec <= V) {
+    *reinterpret_cast<u32x4_any*>(x + col) = Elem<DTYPE>::pack(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (col + i < V) x[col + i] = Elem<DTYPE>::down(v[i]);
+  }
+}
+
+// Running statistics of a soft-max over part of a row, all relative to the maximum m so far:
+// s = sum exp((x - m) / tau), w = sum exp((x - m) / tau) * (x - m).  Parts join in any tree of
+// a fixed shape, so a row's result does not depend on timing.
+//   log-sum-exp = m / tau + ln s,   entropy = ln s - w / (tau s)
+// m starts at the lowest float instead of -inf, so that x - m is defined for a part of -inf
+// alone (its s stays 0).  A NaN, and the inf - inf of an infinite maximum, end in s and stay.
+struct RowStats {
+  float m, s, w;
+};
+
+__device__ __forceinline__ RowStats row_stats_empty() { return {-3.4028234663852886e38f, 0.f, 0.f}; }
+
+__device__ __forceinline__ RowStats row_stats_join(const RowStats& a, const RowStats& b, float rate) {
+  RowStats r;
+  r.m = fmaxf(a.m, b.m);
+  const float da = fmaxf(a.m - r.m, kFarBelow), db = fmaxf(b.m - r.m, kFarBelow);
+  const float fa = __builtin_amdgcn_exp2f(da * rate), fb = __builtin_amdgcn_exp2f(db * rate);
+  r.s = a.s * fa + b.s * fb;
+  r.w = fa * (a.w + a.s * da) + fb * (b.w + b.s * db);
+  return r;
+}
+
+// Adds n elements; rate = log2(e) / tau.
+template <int n>
+__device__ __forceinline__ void row_stats_add(RowStats& a, const float (&x)[n], float rate) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < n; ++i) top = fmaxf(top, x[i]);
+  const float m = fmaxf(a.m, top);
+  const float d = fmaxf(a.m - m, kFarBelow);
+  const float f = __builtin_amdgcn_exp2f(d * rate);
+  a.w = f * (a.w + a.s * d);
+  a.s *= f;
+  a.m = m;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const float di = x[i] - m;
+    const float e = __builtin_amdgcn_exp2f(di * rate);
+    a.s += e;
+    a.w += e * fmaxf(di, kFarBelow);
+  }
+}
+
+__device__ __forceinline__ RowStats row_stats_wave(RowStats a, float rate) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const RowStats o = {__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64), __shfl_xor(a.w, d, 64)};
+    a = row_stats_join(a, o, rate);
+  }
+  return a;
+}
+
+// Over a workgroup of WAVES waves; every thread gets the result.  s_part: WAVES entries of LDS.
+template <int WAVES>
+__device__ __forceinline__ RowStats row_stats_block(RowStats a, float rate, RowStats* s_part) {
+  a = row_stats_wave(a, rate);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = s_part[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) a = row_stats_join(a, s_part[i], rate);
+  }
+  return a;
+}
+
+// Order of the alternatives: by value, then by the lower column; -0 and +0 are equal, and a NaN
+// counts as -inf.  A larger key is a better alternative and no two columns share one.
+__device__ __forceinline__ unsigned long long rank_key(float v, int col) {
+  const float z = v == v ? v + 0.f : -INFINITY;
+  const uint32_t u = __float_as_uint(z);
+  const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((unsigned long long)k << 32) | (0xffffffffu - (uint32_t)col);
+}
+__device__ __forceinline__ int rank_col(unsigned long long key) {
+  return (int)(0xffffffffu - (uint32_t)key);
+}
+
+#endif  // __HIPCC__
+
+}  // namespace icap

@@ -50,15 +50,21 @@ def _call(name, *args):
         return _lib.call(name, *args)
 
 
-def _chk(t, dtype, name):
+def _chk(t, dtype, name, rows=False):
+    """The data pointer of a checked operand.  dtype: the element type asked for, or DTYPES for any
+    of those; rows: only the elements of a row (last axis) have to lie side by side."""
     try:
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s must be a torch.Tensor" % name)
         if not t.is_cuda:
             raise ValueError("%s must live on the GPU (got device %s)" % (name, t.device))
-        if t.dtype != dtype:
-            raise TypeError("%s must be %s (got %s)" % (name, dtype, t.dtype))
-        if not t.is_contiguous():
+        if t.dtype not in dtype if dtype is DTYPES else t.dtype != dtype:
+            raise TypeError("%s must be %s (got %s)" % (
+                name, " or ".join(map(str, DTYPES)) if dtype is DTYPES else dtype, t.dtype))
+        if rows:
+            if not t.dim() or (t.stride(-1) != 1 and t.shape[-1] != 1):
+                raise ValueError("%s must have contiguous rows" % name)
+        elif not t.is_contiguous():
             raise ValueError("%s must be contiguous" % name)
     except Exception:
         _pending().clear()
@@ -82,6 +88,7 @@ def _opt(t, dtype, name):
 
 
 f32, i32, u8 = torch.float32, torch.int32, torch.uint8
+DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
 def dense(x, kernel, bias=None, act=ACT_NONE, out=None):
@@ -379,6 +386,169 @@ def sample_categorical(logits, u, step=0, row_len=None, start_token=-1, eos_toke
     _call("icap_sample_categorical_f32", _chk(logits, f32, "logits"), _chk(u, f32, "u"),
               _opt(row_len, i32, "row_len"), int(step), int(start_token), int(eos_token),
               int(pad_token), _chk(out, i32, "out"), N, V, current_stream())
+    return out
+
+
+# ---- scoring tokens, distillation, embedding gradient ----------------------------------
+#
+# Forward and gradient are calls of their own, as everywhere in this module (torch supplies memory
+# and streams, not the graph of a backward pass).
+
+def _row_split(t, name):
+    """(rows_inner, ld, ld_outer) of a tensor [..., V] with contiguous rows: see icap.h."""
+    V = t.shape[-1]
+    if t.dim() == 1 or t.is_contiguous():
+        return max(1, t.numel() // max(1, V)), V, 0
+    if t.dim() == 2:
+        return max(1, t.shape[0]), t.stride(0), 0
+    if t.dim() == 3:
+        return max(1, t.shape[1]), t.stride(1), t.stride(0)
+    raise ValueError("%s: only [N,V] and [B,T,V] may have rows apart from each other" % name)
+
+
+def _extent(t):
+    """First byte and end of the memory a tensor reaches."""
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _grad_out(out, like, name):
+    """The gradient's tensor: a new one, or the caller's if it fits - the logits themselves, or
+    memory apart from them."""
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError("%s: out must have the logits' shape and dtype" % name)
+    if out.numel() and not (out.data_ptr() == like.data_ptr() and out.stride() == like.stride()):
+        (a, a_end), (b, b_end) = _extent(out), _extent(like)
+        if out.device == like.device and a < b_end and b < a_end:
+            raise ValueError("%s: out overlaps the logits without being them" % name)
+    return out
+
+
+def _row_strides(t, out):
+    """(rows_inner, ld, ld_outer, out_ld, out_ld_outer): the rows of two tensors of one shape, split
+    the same way."""
+    split, out_split = _row_split(t, "logits"), _row_split(out, "out")
+    if t.dim() == 3 and split[0] != out_split[0]:      # one of them is contiguous: split it too
+        split, out_split = ((max(1, s.shape[1]), s.stride(1), s.stride(0)) for s in (t, out))
+    return (*split, *out_split[1:])
+
+
+def token_log_probs(logits, tokens, top_k=0, pad_token=-1):
+    """Log probabilities of `tokens` [...] int32 under the softmax of `logits` [..., V] (float32,
+    bfloat16 or float16) -> (log_probs [...], entropy [...], stats [..., 2], top_ids [..., top_k],
+    top_log_probs [..., top_k]); float32 and int32, the last two None with top_k = 0.
+
+    stats holds each row's maximum and the log of its sum of exponentials above it (their sum is
+    the log-sum-exp): token_log_probs_grad takes it.  The alternatives come in descending order,
+    equal logits by the lower id.  Rows whose token is pad_token are left out: zeros, ids of -1."""
+    if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
+        raise ValueError("token_log_probs: logits must be [..., V] for tokens [...]")
+    V, N, dev, shape, top_k = logits.shape[-1], tokens.numel(), logits.device, tokens.shape, int(top_k)
+    if not 0 <= top_k <= min(V, _lib.MAX_ALTERNATIVES):
+        raise ValueError("token_log_probs: top_k must be in 0 .. min(V, %d)" % _lib.MAX_ALTERNATIVES)
+    log_probs = torch.empty(shape, dtype=f32, device=dev)
+    entropy = torch.empty(shape, dtype=f32, device=dev)
+    stats = torch.empty(*shape, 2, dtype=f32, device=dev)
+    top_ids = torch.empty(*shape, top_k, dtype=i32, device=dev) if top_k else None
+    top_lp = torch.empty(*shape, top_k, dtype=f32, device=dev) if top_k else None
+    x, t = _chk(logits, DTYPES, "logits", rows=True), _chk(tokens, i32, "tokens")
+    if N:
+        _call("icap_token_log_probs", x, DTYPES[logits.dtype], N, V, *_row_split(logits, "logits"), t,
+              int(pad_token), top_k, log_probs.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+              top_ids.data_ptr() if top_k else None, top_lp.data_ptr() if top_k else None,
+              current_stream())
+    return log_probs, entropy, stats, top_ids, top_lp
+
+
+def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, grad_entropy=None,
+                         pad_token=-1, out=None):
+    """Gradient to the logits of sum(grad_log_probs * log_probs + grad_entropy * entropy), with the
+    stats and entropy that token_log_probs returned for the same logits; either gradient may be
+    None.  [..., V] in the logits' dtype; out=logits overwrites them."""
+    if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
+        raise ValueError("token_log_probs_grad: logits must be [..., V] for tokens [...]")
+    if stats.shape != (*tokens.shape, 2) or entropy.shape != tokens.shape:
+        raise ValueError("token_log_probs_grad: stats must be [..., 2] and entropy [...] for tokens [...]")
+    for g in (grad_log_probs, grad_entropy):
+        if g is not None and g.shape != tokens.shape:
+            raise ValueError("token_log_probs_grad: gradients must have the tokens' shape")
+    V, N = logits.shape[-1], tokens.numel()
+    out = _grad_out(out, logits, "token_log_probs_grad")
+    args = (_chk(logits, DTYPES, "logits", rows=True), _chk(out, DTYPES, "out", rows=True),
+            _chk(tokens, i32, "tokens"), _chk(stats, f32, "stats"), _chk(entropy, f32, "entropy"),
+            _opt(grad_log_probs, f32, "grad_log_probs"), _opt(grad_entropy, f32, "grad_entropy"))
+    if N and V:
+        inner, ld, ld_outer, out_ld, out_ld_outer = _row_strides(logits, out)
+        _call("icap_token_log_probs_grad", args[0], DTYPES[logits.dtype], N, V, inner, ld, ld_outer, args[2],
+              int(pad_token), *args[3:], args[1], out_ld, out_ld_outer, current_stream())
+    return out
+
+
+def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss=None, out=None):
+    """Distillation from a teacher's best logits: logits [..., V], teacher_logits and teacher_ids
+    (int32) [..., K] -> (loss [...], dlogits or None).
+
+    loss = temperature^2 * KL(softmax(teacher_logits / temperature) over the K entries ||
+    softmax(logits / temperature)).  With grad_loss [...] also the gradient of
+    sum(grad_loss * loss) to the logits, [..., V] in their dtype, in the same call (out=logits
+    overwrites them).  An entry with id -1 is absent; a row without entries gives zeros."""
+    if logits.dim() == 0 or teacher_ids.dim() == 0 or teacher_ids.shape[:-1] != logits.shape[:-1] or \
+            teacher_logits.shape != teacher_ids.shape:
+        raise ValueError("distill_loss: teacher_logits and teacher_ids must be [..., K] for logits [..., V]")
+    shape, V, K = logits.shape[:-1], logits.shape[-1], teacher_ids.shape[-1]
+    if not 1 <= K <= _lib.MAX_TEACHER_LOGITS:
+        raise ValueError("distill_loss: the teacher must hand over 1 .. %d logits" % _lib.MAX_TEACHER_LOGITS)
+    if grad_loss is not None and grad_loss.shape != shape:
+        raise ValueError("distill_loss: grad_loss must have one value per row of the logits")
+    if grad_loss is None and out is not None:
+        raise ValueError("distill_loss: out needs grad_loss")
+    loss = torch.empty(shape, dtype=f32, device=logits.device)
+    N = loss.numel()
+    x, tx = _chk(logits, DTYPES, "logits", rows=True), _chk(teacher_logits, DTYPES, "teacher_logits")
+    ti, gl = _chk(teacher_ids, i32, "teacher_ids"), _opt(grad_loss, f32, "grad_loss")
+    g = None
+    if grad_loss is not None:
+        out = _grad_out(out, logits, "distill_loss")
+        g = _chk(out, DTYPES, "out", rows=True)
+    if N and V:
+        inner, ld, ld_outer, out_ld, out_ld_outer = _row_strides(logits, logits if out is None else out)
+        _call("icap_distill_loss", x, DTYPES[logits.dtype], N, V, inner, ld, ld_outer, tx,
+              DTYPES[teacher_logits.dtype], ti, K, float(temperature), gl, loss.data_ptr(), g, out_ld,
+              out_ld_outer, current_stream())
+    return loss, out
+
+
+def embedding_scaled(table, ids, scale=1.0, pad_token=-1):
+    """scale * table[ids]: table [V,D] (float32, bfloat16 or float16), ids [...] int32 -> [..., D] in
+    the table's dtype; zero rows for pad_token and for ids outside the table."""
+    V, D = table.shape
+    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
+    tab, i = _chk(table, DTYPES, "table"), _chk(ids, i32, "ids")
+    if out.numel():
+        _call("icap_embedding_scaled", tab, DTYPES[table.dtype], i, out.data_ptr(), ids.numel(), V, D,
+              float(scale), int(pad_token), current_stream())
+    return out
+
+
+def embedding_grad(grad, ids, vocab_size, scale=1.0, pad_token=-1):
+    """Gradient of embedding_scaled to its table: grad [..., D], ids [...] -> [vocab_size, D] in grad's
+    dtype.  Sums run in float32 in an order the ids alone decide: the same inputs, the same bits."""
+    if grad.dim() == 0 or grad.shape[:-1] != ids.shape:
+        raise ValueError("embedding_grad: grad must be [..., D] for ids [...]")
+    V, D, N, dev = int(vocab_size), grad.shape[-1], ids.numel(), grad.device
+    if V < 1:
+        raise ValueError("embedding_grad: vocab_size must be positive")
+    out = torch.empty(V, D, dtype=grad.dtype, device=dev)
+    g, i = _chk(grad, DTYPES, "grad"), _chk(ids, i32, "ids")
+    if N == 0:
+        return out.zero_()
+    if D:
+        need = int(_lib.load().icap_embedding_grad_workspace_bytes(N, V, D))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _call("icap_embedding_grad", g, DTYPES[grad.dtype], i, out.data_ptr(), N, V, D, float(scale),
+              int(pad_token), ws.data_ptr(), need, current_stream())
     return out
 
 

@@ -52,6 +52,14 @@ extern "C" {
 
 #define ICAP_MAX_BEAM_WIDTH 16
 
+/* Element types of the operators that take more than fp32 (logits, embedding tables). */
+#define ICAP_DTYPE_F32 0
+#define ICAP_DTYPE_BF16 1
+#define ICAP_DTYPE_F16 2
+
+#define ICAP_MAX_ALTERNATIVES 32   /* top_k of icap_token_log_probs */
+#define ICAP_MAX_TEACHER_LOGITS 256 /* K of icap_distill_loss */
+
 typedef void* icap_stream_t;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -561,6 +569,74 @@ int icap_engine_kernel_times(icap_engine* engine, float* ms /*[ICAP_K_COUNT]*/,
 int icap_sample_categorical_f32(const float* logits, const float* u, const int32_t* row_len,
                                 int step, int start_token, int eos_token, int pad_token,
                                 int32_t* samples, int N, int V, icap_stream_t stream);
+
+/* ---- what a decoder is trained with ---------------------------------------------------
+ * The reference trains its decoders in TensorFlow (teacher forcing recurrent_example.py:381-475,
+ * REINFORCE / self-critical / actor-critic utils/train_utils.py:397-515 on the samples of
+ * utils/agent_utils.py); these are the operators at the two ends of such a step, forward and
+ * gradient, plus distillation.  `dtype` is the ICAP_DTYPE_* of the logits (table), statistics
+ * and losses are float32.  Logits are rows of V elements: row r starts at element
+ *   (r / rows_inner) * ld_outer + (r % rows_inner) * ld
+ * of `logits` (rows_inner >= N: a matrix of leading dimension ld; rows_inner = T - 1: the first
+ * T - 1 positions of a [B,T,V] tensor), at any element alignment.  A logit of -inf takes no part;
+ * a row of nothing else has no distribution.  NaN or +inf in a row makes its floating results NaN. */
+
+/* Log probabilities of given tokens with the entropy of their rows and the best alternatives.
+ *   p_j = exp(x_j) / sum_i exp(x_i);  log_probs[n] = log p_tokens[n];
+ *   entropy[n] = -sum_j p_j log p_j;  stats[n] = (max_j x_j, log sum_j exp(x_j - max)), whose sum
+ *   is the log-sum-exp;  top_ids / top_log_probs[n, 0..top_k): the top_k largest, in descending
+ *   order, equal logits by the lower id (a NaN last).
+ * A row whose token is pad_token is not read: zeros, ids of -1.  Any other token outside [0,V)
+ * gives log_probs NaN.  Row without a distribution: log_probs -inf, entropy 0, stats (-inf, 0),
+ * top_log_probs -inf.  top_k <= min(V, ICAP_MAX_ALTERNATIVES); 0 needs no top_* arrays. */
+int icap_token_log_probs(const void* logits, int dtype, int N, int V, int rows_inner, long long ld,
+                         long long ld_outer, const int32_t* tokens, int pad_token, int top_k,
+                         float* log_probs, float* entropy, float* stats, int32_t* top_ids,
+                         float* top_log_probs, icap_stream_t stream);
+
+/* Gradient of sum_n (grad_log_probs[n] log_probs[n] + grad_entropy[n] entropy[n]) to the logits:
+ *   dlogits[n,j] = grad_log_probs[n] ([j = tokens[n]] - p_j) - grad_entropy[n] p_j (log p_j + entropy[n])
+ * with stats and entropy as icap_token_log_probs wrote them; either gradient may be NULL (zero).
+ * Rows of pad_token, without a distribution, or with both gradients zero are zeros and are not
+ * read.  dlogits has the logits' dtype and row split, its own strides, and may be the logits
+ * themselves (same strides). */
+int icap_token_log_probs_grad(const void* logits, int dtype, int N, int V, int rows_inner, long long ld,
+                              long long ld_outer, const int32_t* tokens, int pad_token,
+                              const float* stats, const float* entropy, const float* grad_log_probs,
+                              const float* grad_entropy, void* dlogits, long long out_ld,
+                              long long out_ld_outer, icap_stream_t stream);
+
+/* Distillation from a teacher's K best logits per row, teacher_logits[N,K] at teacher_ids[N,K]:
+ *   q = softmax over the K entries of teacher_logits / temperature,  p = softmax(x / temperature),
+ *   loss[n] = temperature^2 * sum_k q_k (log q_k - log p_id(k))
+ * and, with grad_loss, the gradient of sum_n grad_loss[n] loss[n] in the same call:
+ *   dlogits[n,j] = grad_loss[n] * temperature * (p_j - sum over k with id(k) = j of q_k)
+ * (dlogits as in icap_token_log_probs_grad; both NULL for the loss alone).  An entry with id -1
+ * or a logit of -inf is absent; a row without entries has loss 0 and a zero gradient and its
+ * logits are not read.  An id otherwise outside [0,V) makes the row NaN.  grad_loss[n] = 0 gives
+ * a zero gradient.  Row without a distribution: loss +inf where the teacher has entries, zero
+ * gradient.  K <= ICAP_MAX_TEACHER_LOGITS, temperature in 0.001 .. 1000. */
+int icap_distill_loss(const void* logits, int dtype, int N, int V, int rows_inner, long long ld,
+                      long long ld_outer, const void* teacher_logits, int teacher_dtype,
+                      const int32_t* teacher_ids, int K, float temperature, const float* grad_loss,
+                      float* loss, void* dlogits, long long out_ld, long long out_ld_outer,
+                      icap_stream_t stream);
+
+/* out[N,D] = scale * table[ids[n], :], rounded once; a zero row where ids[n] is pad_token or
+ * outside [0,V).  icap_embedding_f32 with a factor, a padding token and 16-bit tables. */
+int icap_embedding_scaled(const void* table, int dtype, const int32_t* ids, void* out, int N, int V,
+                          int D, float scale, int pad_token, icap_stream_t stream);
+
+/* Its gradient: dtable[V,D] = scale * sum over n with ids[n] = v of grad[n, :], every row written
+ * (zeros where no token asks for it), tokens that are pad_token or outside [0,V) left out.  The
+ * positions are sorted by token and summed in float32 in an order that depends on the ids alone:
+ * the same inputs give the same bits.  workspace: 16-byte aligned, of the size that
+ * icap_embedding_grad_workspace_bytes gives (0: bad shape); its contents need no initialisation
+ * and mean nothing afterwards. */
+size_t icap_embedding_grad_workspace_bytes(int N, int V, int D);
+int icap_embedding_grad(const void* grad, int dtype, const int32_t* ids, void* dtable, int N, int V,
+                        int D, float scale, int pad_token, void* workspace, size_t workspace_bytes,
+                        icap_stream_t stream);
 
 /* ---- transformer decoder path ------------------------------------------------------
  * decoder/transform_decoder.py + attention/attention.py:160-562 + decoder/ffn_layer.py +
