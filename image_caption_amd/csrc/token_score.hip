@@ -8,6 +8,7 @@ namespace icap {
 namespace {
 
 constexpr int NT = 256;
+constexpr int kCandidates = 256;
 
 struct ScoreArgs {
   const void* logits;
@@ -19,12 +20,102 @@ struct ScoreArgs {
   float* top_log_probs;
 };
 
-// One workgroup per row, one pass for the statistics and one more per alternative.
-template <int DTYPE>
-__global__ __launch_bounds__(NT) void token_log_probs_kernel(ScoreArgs p) {
+template <int WAVES>
+struct TopScratch {
+  float lane_max[WAVES][64];
+  int piece[kCandidates];
+  unsigned long long key[kCandidates];
+  unsigned long long best[WAVES];
+  int pieces, count;
+};
+
+// The k best columns of a row, best first, handed to out(rank, key).  `top` is the thread's own
+// maximum.  The workgroup's lanes form 64 groups (same lane, all waves); the k-th largest of the 64
+// group maxima is a value that at least k elements reach, so everything below it is out of the
+// question: some tens of candidates are left for any k up to 32, and threads whose own maximum is
+// lower do not look at their elements again.  Pieces that reach the bound are noted in LDS, their
+// elements shared out over the threads, the candidates noted in any order, and each finds its
+// rank by counting the better ones.  Rows where too many elements tie with the bound, or with
+// fewer than k elements over -inf, take one round over the row for each alternative.
+template <int DTYPE, int WAVES, int NV, class Out>
+__device__ __forceinline__ void top_columns(const Row<DTYPE, WAVES, NV>& row, float top, int k,
+                                            TopScratch<WAVES>& s, Out out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float group = top;
+  if (tid == 0) s.pieces = s.count = 0;
+  if constexpr (WAVES > 1) {
+    s.lane_max[wave][lane] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) group = fmaxf(group, s.lane_max[w][lane]);
+  } else {
+    __syncthreads();
+  }
+  // the k-th largest of 64, bit by bit, until exactly k reach the bound
+  const uint32_t mine = order_of(group);
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = bound | (1u << bit);
+    const int reach = __popcll(__ballot(mine >= next));
+    if (reach >= k) bound = next;
+    if (reach == k) break;
+  }
+  const float least = order_value(bound);
+  if (top >= least)
+    row.each([&](const auto& v, int c) {
+      if (row_max(-INFINITY, v) < least) return;
+      const int at = atomicAdd(&s.pieces, 1);
+      if (at < kCandidates) s.piece[at] = c;
+    });
+  __syncthreads();
+  constexpr int n = Elem<DTYPE>::kVec;
+  const int noted = s.pieces;
+  if (noted <= kCandidates)
+    for (int i = tid; i < noted * n; i += WAVES * 64) {
+      const int c0 = s.piece[i / n], c = c0 + i % n;
+      if (c0 >= row.pieces * n && i % n) continue;      // a single element behind the last piece
+      const float v = Elem<DTYPE>::up(row.x[c]);
+      if (!(v >= least)) continue;
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kCandidates) s.key[at] = rank_key(v, c);
+    }
+  __syncthreads();
+  const int count = s.count;
+  if (noted <= kCandidates && count >= k && count <= kCandidates) {
+    for (int i = tid; i < count; i += WAVES * 64) {
+      const unsigned long long key = s.key[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += s.key[j] > key;
+      if (rank < k) out(rank, key);
+    }
+    return;
+  }
+  unsigned long long below = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    unsigned long long best = 0;
+    for (int c = tid; c < row.V; c += WAVES * 64) {
+      const unsigned long long key = rank_key(Elem<DTYPE>::up(row.x[c]), c);
+      if (key < below && key > best) best = key;
+    }
+    for (int d = 32; d > 0; d >>= 1) best = max(best, (unsigned long long)__shfl_xor(best, d, 64));
+    if constexpr (WAVES > 1) {
+      __syncthreads();
+      if (lane == 0) s.best[wave] = best;
+      __syncthreads();
+      best = s.best[lane & (WAVES - 1)];
+      for (int d = WAVES / 2; d > 0; d >>= 1) best = max(best, (unsigned long long)__shfl_xor(best, d, 64));
+    }
+    below = best;
+    if (tid == 0) out(r, best);
+  }
+}
+
+// One workgroup per row.
+template <int DTYPE, int WAVES, int NV>
+__global__ __launch_bounds__(WAVES * 64) void token_log_probs_kernel(ScoreArgs p) {
   typedef Elem<DTYPE> E;
-  __shared__ RowStats s_part[NT / 64];
-  __shared__ unsigned long long s_key[NT / 64];
+  __shared__ RowStats s_part[WAVES];
+  __shared__ TopScratch<WAVES> s_top;
   const int row = blockIdx.y * gridDim.x + blockIdx.x, tid = threadIdx.x;
   if (row >= p.N) return;
   const int token = p.tokens[row];
@@ -34,52 +125,34 @@ __global__ __launch_bounds__(NT) void token_log_probs_kernel(ScoreArgs p) {
       p.entropy[row] = 0.f;
       p.stats[2 * (size_t)row] = p.stats[2 * (size_t)row + 1] = 0.f;
     }
-    for (int i = tid; i < p.k; i += NT) {
-      p.top_ids[(size_t)row * p.k + i] = -1;
-      p.top_log_probs[(size_t)row * p.k + i] = 0.f;
+    if (tid < p.k) {
+      p.top_ids[(size_t)row * p.k + tid] = -1;
+      p.top_log_probs[(size_t)row * p.k + tid] = 0.f;
     }
     return;
   }
   const typename E::type* x = (const typename E::type*)p.logits + p.view.at(row);
-  RowStats a = row_stats_empty();
-  for (int c = tid * E::kVec; c < p.V; c += NT * E::kVec) {
-    float v[E::kVec];
-    load_vec<DTYPE>(x, c, p.V, -INFINITY, v);
-    row_stats_add(a, v, kLog2e);
-  }
-  a = row_stats_block<NT / 64>(a, kLog2e, s_part);
+  Row<DTYPE, WAVES, NV> data;
+  data.open(x, p.V);
+  const bool inside = token >= 0 && token < p.V;
+  const float x_t = inside ? E::up(x[token]) : NAN;
+  const RowStats part = data.stats(kLog2e);
+  const RowStats a = row_stats_block<WAVES>(part, kLog2e, s_part);
   const bool none = a.s == 0.f;                 // every logit is -inf
   const float m = none ? -INFINITY : a.m;
   const float log_s = none ? 0.f : logf(a.s);
   if (tid == 0) {
-    float lp;
-    if (token < 0 || token >= p.V) lp = NAN;
-    else if (none) lp = -INFINITY;
-    else lp = (E::up(x[token]) - m) - log_s;
-    p.log_probs[row] = lp;
+    p.log_probs[row] = inside && none ? -INFINITY : (x_t - m) - log_s;
     p.entropy[row] = none ? 0.f : log_s - a.w / a.s;
     p.stats[2 * (size_t)row] = m;
     p.stats[2 * (size_t)row + 1] = log_s;
   }
-  unsigned long long below = ~0ull;
-  for (int i = 0; i < p.k; ++i) {
-    unsigned long long best = 0;
-    for (int c = tid; c < p.V; c += NT) {
-      const unsigned long long key = rank_key(E::up(x[c]), c);
-      if (key < below && key > best) best = key;
-    }
-    for (int d = 32; d > 0; d >>= 1) best = max(best, (unsigned long long)__shfl_xor(best, d, 64));
-    __syncthreads();
-    if ((tid & 63) == 0) s_key[tid >> 6] = best;
-    __syncthreads();
-    for (int w = 0; w < NT / 64; ++w) best = max(best, s_key[w]);
-    below = best;
-    if (tid == 0) {
-      const int col = rank_col(best);
-      p.top_ids[(size_t)row * p.k + i] = col;
-      p.top_log_probs[(size_t)row * p.k + i] = none ? -INFINITY : (E::up(x[col]) - m) - log_s;
-    }
-  }
+  if (p.k == 0) return;
+  top_columns(data, part.m, p.k, s_top, [&](int rank, unsigned long long key) {
+    const int col = rank_col(key);
+    p.top_ids[(size_t)row * p.k + rank] = col;
+    p.top_log_probs[(size_t)row * p.k + rank] = none ? -INFINITY : (E::up(x[col]) - m) - log_s;
+  });
 }
 
 struct ScoreGradArgs {
@@ -90,39 +163,61 @@ struct ScoreGradArgs {
   const float *stats, *entropy, *g_lp, *g_h;
   void* out;
   RowView out_view;
+  int shares;      // of a row
 };
 
 // d log p_t / d x_j = [j = t] - p_j,   d H / d x_j = -p_j (log p_j + H)
+// Element by element, so a row is cut into shares of kGradPieces pieces a thread.
+constexpr int kGradPieces = 4;
+
 template <int DTYPE>
 __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs p) {
   typedef Elem<DTYPE> E;
-  const int row = blockIdx.y * gridDim.x + blockIdx.x, tid = threadIdx.x;
-  if (row >= p.N) return;
+  typedef typename E::type type;
+  const int row = blockIdx.x / p.shares, share = blockIdx.x % p.shares, tid = threadIdx.x;
   const int token = p.tokens[row];
-  const typename E::type* x = (const typename E::type*)p.logits + p.view.at(row);
-  typename E::type* g = (typename E::type*)p.out + p.out_view.at(row);
+  const type* x = (const type*)p.logits + p.view.at(row);
+  type* g = (type*)p.out + p.out_view.at(row);
   float g_lp = p.g_lp ? p.g_lp[row] : 0.f;
   const float g_h = p.g_h ? p.g_h[row] : 0.f;
   const float m = p.stats[2 * (size_t)row], log_s = p.stats[2 * (size_t)row + 1], h = p.entropy[row];
+  const int pieces = p.V / E::kVec, first = share * NT * kGradPieces + tid;
+  const int tail = pieces * E::kVec + tid;
+  const bool has_tail = share == p.shares - 1 && tail < p.V;
   if (token == p.pad || m == -INFINITY || (g_lp == 0.f && g_h == 0.f)) {
     const float zero[E::kVec] = {};
-    for (int c = tid * E::kVec; c < p.V; c += NT * E::kVec) store_vec<DTYPE>(g, c, p.V, zero);
+#pragma unroll
+    for (int j = 0; j < kGradPieces; ++j)
+      if (first + j * NT < pieces) Piece<DTYPE, E::kVec>::store(g + (size_t)(first + j * NT) * E::kVec, zero);
+    if (has_tail) g[tail] = E::down(0.f);
     return;
   }
   if ((token < 0 || token >= p.V) && g_lp != 0.f) g_lp = NAN;
   const float inv_s = __builtin_amdgcn_exp2f(-log_s * kLog2e);
-  for (int c = tid * E::kVec; c < p.V; c += NT * E::kVec) {
-    float v[E::kVec];
-    load_vec<DTYPE>(x, c, p.V, -INFINITY, v);
+  auto grad = [&](float v, int c) {
+    const float d = v - m;
+    const float e = __builtin_amdgcn_exp2f(d * kLog2e) * inv_s;
+    const float u = fmaxf(d, kFarBelow) - log_s + h;
+    return -e * (g_lp + g_h * u) + (c == token ? g_lp : 0.f);
+  };
+  u32x4 raw[kGradPieces];
+  float t = 0.f;
+  if (has_tail) t = E::up(x[tail]);
 #pragma unroll
-    for (int i = 0; i < E::kVec; ++i) {
-      const float d = v[i] - m;
-      const float e = __builtin_amdgcn_exp2f(d * kLog2e) * inv_s;
-      const float u = fmaxf(d, kFarBelow) - log_s + h;
-      v[i] = -e * (g_lp + g_h * u) + (c + i == token ? g_lp : 0.f);
-    }
-    store_vec<DTYPE>(g, c, p.V, v);
+  for (int j = 0; j < kGradPieces; ++j)
+    if (pieces > 0)
+      raw[j] = *reinterpret_cast<const u32x4_any*>(x + (size_t)min(first + j * NT, pieces - 1) * E::kVec);
+#pragma unroll
+  for (int j = 0; j < kGradPieces; ++j) {
+    const int i = first + j * NT;
+    if (i >= pieces) break;
+    float v[E::kVec];
+    E::unpack(raw[j], v);
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) v[e] = grad(v[e], i * E::kVec + e);
+    Piece<DTYPE, E::kVec>::store(g + (size_t)i * E::kVec, v);
   }
+  if (has_tail) g[tail] = E::down(grad(t, tail));
 }
 
 constexpr int kMaxTeacher = ICAP_MAX_TEACHER_LOGITS;
@@ -149,10 +244,10 @@ __device__ __forceinline__ float load_typed(const void* p, int dtype, size_t i) 
 
 // loss = tau^2 sum_k q_k (log q_k - log p[id_k]),  q = soft-max of the teacher's K logits at tau,
 // p = soft-max of the row at tau;   d loss / d x_j = tau (p_j - sum over k with id_k = j of q_k)
-template <int DTYPE>
-__global__ __launch_bounds__(NT) void distill_loss_kernel(DistillArgs p) {
+template <int DTYPE, int WAVES, int NV>
+__global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p) {
   typedef Elem<DTYPE> E;
-  __shared__ RowStats s_part[NT / 64];
+  __shared__ RowStats s_part[WAVES];
   __shared__ int s_id[kMaxTeacher];
   __shared__ float s_q[kMaxTeacher], s_log_q[kMaxTeacher], s_x[kMaxTeacher];
   __shared__ int s_alive, s_bad;
@@ -196,19 +291,12 @@ __global__ __launch_bounds__(NT) void distill_loss_kernel(DistillArgs p) {
   const float coef = p.g_loss ? p.g_loss[row] * p.tau : 0.f;
   if (!s_alive && !s_bad) {
     if (tid == 0) p.loss[row] = 0.f;
-    if (g) {
-      const float zero[E::kVec] = {};
-      for (int c = tid * E::kVec; c < p.V; c += NT * E::kVec) store_vec<DTYPE>(g, c, p.V, zero);
-    }
+    if (g) write_zeros<DTYPE, WAVES>(g, p.V);
     return;
   }
-  RowStats a = row_stats_empty();
-  for (int c = tid * E::kVec; c < p.V; c += NT * E::kVec) {
-    float v[E::kVec];
-    load_vec<DTYPE>(x, c, p.V, -INFINITY, v);
-    row_stats_add(a, v, rate);
-  }
-  a = row_stats_block<NT / 64>(a, rate, s_part);
+  Row<DTYPE, WAVES, NV> data;
+  data.open(x, p.V);
+  const RowStats a = row_stats_block<WAVES>(data.stats(rate), rate, s_part);
   const bool none = a.s == 0.f;
   const float log_s = logf(a.s), inv_s = 1.f / a.s;
   if (tid < 64) {
@@ -222,20 +310,16 @@ __global__ __launch_bounds__(NT) void distill_loss_kernel(DistillArgs p) {
     if (tid == 0) p.loss[row] = s_bad ? NAN : sum;
   }
   if (!g) return;
-  const bool zero_row = coef == 0.f || (none && !s_bad);
-  const float c0 = zero_row ? 0.f : s_bad ? NAN : coef;
-  for (int c = tid * E::kVec; c < p.V; c += NT * E::kVec) {
-    float v[E::kVec];
-    load_vec<DTYPE>(x, c, p.V, -INFINITY, v);
-#pragma unroll
-    for (int i = 0; i < E::kVec; ++i)
-      v[i] = zero_row ? 0.f : c0 * (__builtin_amdgcn_exp2f((v[i] - a.m) * rate) * inv_s);
-    store_vec<DTYPE>(g, c, p.V, v);
+  if (coef == 0.f || (none && !s_bad)) {
+    write_zeros<DTYPE, WAVES>(g, p.V);
+    return;
   }
-  if (zero_row || s_bad) return;
+  const float c0 = s_bad ? NAN : coef;
+  data.write(g, [&](float v, int) { return c0 * (__builtin_amdgcn_exp2f((v - a.m) * rate) * inv_s); });
+  if (s_bad) return;
   __syncthreads();
   // the teacher's columns again, the first of several entries with the same id for all of them
-  for (int k = tid; k < p.K; k += NT) {
+  for (int k = tid; k < p.K; k += WAVES * 64) {
     const int id = s_id[k];
     bool first = id >= 0;
     float q = 0.f;
@@ -248,6 +332,8 @@ __global__ __launch_bounds__(NT) void distill_loss_kernel(DistillArgs p) {
       g[id] = E::down(c0 * (__builtin_amdgcn_exp2f((s_x[k] - a.m) * rate) * inv_s - q));
   }
 }
+
+constexpr long long kMostBlocks = (1LL << 32) / 1024 - 1;      // a launch counts 2^32 lanes along x
 
 dim3 row_grid(int N) {
   const int x = N < 65536 ? N : 65536;
@@ -275,6 +361,39 @@ int check_out(const char* what, int N, int V, const RowView& v) {
   return ICAP_OK;
 }
 
+// Waves for a row and pieces a thread holds.  A row goes to as few waves as keep it in registers
+// (their joins cost more, the more there are), and to a large workgroup where rows are few and each
+// should be done soon.
+struct RowShape {
+  int waves, held;
+};
+RowShape row_shape(int dtype, int N, int V) {
+  const int pieces = V / (dtype == ICAP_DTYPE_F32 ? 4 : 8);
+  const bool many = N > 512;      // two rows a compute unit
+  if (pieces <= 64 * (many ? 4 : 1)) return {1, 4};
+  if (pieces <= 256 * (many ? 4 : 2)) return {4, 4};
+  if (many && pieces <= 256 * 10) return {4, 10};
+  if (pieces <= 1024 * 4) return {16, 4};
+  if (pieces <= 1024 * 8) return {16, 8};
+  if (pieces <= 1024 * 16) return {16, 16};
+  return {16, 0};
+}
+
+#define ICAP_BY_SHAPE(D, shape, call)                                              \
+  do {                                                                             \
+    if ((shape).waves == 1) call(D, 1, 4);                                         \
+    else if ((shape).waves == 4) { if ((shape).held == 4) call(D, 4, 4); else call(D, 4, 10); } \
+    else if ((shape).held == 4) call(D, 16, 4);                                    \
+    else if ((shape).held == 8) call(D, 16, 8);                                    \
+    else if ((shape).held == 16) call(D, 16, 16);                                  \
+    else call(D, 16, 0);                                                           \
+  } while (0)
+#define ICAP_BY_ROWS(dtype, shape, call)                                           \
+  do {                                                                             \
+    if ((dtype) == ICAP_DTYPE_F32) ICAP_BY_SHAPE(ICAP_DTYPE_F32, shape, call);     \
+    else if ((dtype) == ICAP_DTYPE_BF16) ICAP_BY_SHAPE(ICAP_DTYPE_BF16, shape, call); \
+    else ICAP_BY_SHAPE(ICAP_DTYPE_F16, shape, call);                               \
+  } while (0)
 #define ICAP_BY_DTYPE(dtype, call)                                   \
   do {                                                               \
     if ((dtype) == ICAP_DTYPE_F32) { call(ICAP_DTYPE_F32); }         \
@@ -301,8 +420,10 @@ int icap_token_log_probs(const void* logits, int dtype, int N, int V, int rows_i
   if (top_k > ICAP_MAX_ALTERNATIVES)
     return fail(ICAP_ERR_UNSUPPORTED, "token_log_probs: top_k %d is over %d", top_k, ICAP_MAX_ALTERNATIVES);
   ScoreArgs a{logits, view, tokens, N, V, pad_token, top_k, log_probs, entropy, stats, top_ids, top_log_probs};
-#define LAUNCH(D) hipLaunchKernelGGL(token_log_probs_kernel<D>, row_grid(N), dim3(NT), 0, (hipStream_t)stream, a)
-  ICAP_BY_DTYPE(dtype, LAUNCH);
+  const RowShape shape = row_shape(dtype, N, V);
+#define LAUNCH(D, W, NV)                                                                       \
+  hipLaunchKernelGGL((token_log_probs_kernel<D, W, NV>), row_grid(N), dim3(W * 64), 0, (hipStream_t)stream, a)
+  ICAP_BY_ROWS(dtype, shape, LAUNCH);
 #undef LAUNCH
   ICAP_LAUNCH_CHECK("token_log_probs_kernel");
   return ICAP_OK;
@@ -318,8 +439,13 @@ int icap_token_log_probs_grad(const void* logits, int dtype, int N, int V, int r
   if (int rc = check_rows("token_log_probs_grad", dtype, N, V, view)) return rc;
   if (int rc = check_rows("token_log_probs_grad", dtype, N, V, out)) return rc;
   if (int rc = check_out("token_log_probs_grad", N, V, out)) return rc;
-  ScoreGradArgs a{logits, view, tokens, N, V, pad_token, stats, entropy, grad_log_probs, grad_entropy, dlogits, out};
-#define LAUNCH(D) hipLaunchKernelGGL(token_log_probs_grad_kernel<D>, row_grid(N), dim3(NT), 0, (hipStream_t)stream, a)
+  ScoreGradArgs a{logits, view, tokens, N, V, pad_token, stats, entropy, grad_log_probs, grad_entropy, dlogits, out,
+                  std::max(1, ceil_div(V / (dtype == ICAP_DTYPE_F32 ? 4 : 8), NT * kGradPieces))};
+  const long long blocks = (long long)N * a.shares;
+  if (blocks > kMostBlocks)
+    return fail(ICAP_ERR_UNSUPPORTED, "token_log_probs_grad: %d rows of %d are too many for one call", N, V);
+#define LAUNCH(D)                                                                                   \
+  hipLaunchKernelGGL(token_log_probs_grad_kernel<D>, dim3((unsigned)blocks), dim3(NT), 0, (hipStream_t)stream, a)
   ICAP_BY_DTYPE(dtype, LAUNCH);
 #undef LAUNCH
   ICAP_LAUNCH_CHECK("token_log_probs_grad_kernel");
@@ -347,8 +473,10 @@ int icap_distill_loss(const void* logits, int dtype, int N, int V, int rows_inne
   }
   DistillArgs a{logits, view, teacher_logits, teacher_dtype, teacher_ids, N, V, K, temperature,
                 grad_loss, loss, dlogits, out};
-#define LAUNCH(D) hipLaunchKernelGGL(distill_loss_kernel<D>, row_grid(N), dim3(NT), 0, (hipStream_t)stream, a)
-  ICAP_BY_DTYPE(dtype, LAUNCH);
+  const RowShape shape = row_shape(dtype, N, V);
+#define LAUNCH(D, W, NV)                                                                       \
+  hipLaunchKernelGGL((distill_loss_kernel<D, W, NV>), row_grid(N), dim3(W * 64), 0, (hipStream_t)stream, a)
+  ICAP_BY_ROWS(dtype, shape, LAUNCH);
 #undef LAUNCH
   ICAP_LAUNCH_CHECK("distill_loss_kernel");
   return ICAP_OK;

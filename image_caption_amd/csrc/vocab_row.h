@@ -103,6 +103,27 @@ struct Elem<ICAP_DTYPE_F16> {
   }
 };
 
+// n elements from p on, n = kVec (one 16-byte access) or 1.  No bounds and no branch, so that a
+// batch of loads stays in flight together: the caller keeps col + n inside the row.
+template <int DTYPE, int n>
+struct Piece {
+  typedef typename Elem<DTYPE>::type type;
+  u32x4 raw;
+  __device__ __forceinline__ void load(const type* p) { raw = *reinterpret_cast<const u32x4_any*>(p); }
+  __device__ __forceinline__ void unpack(float (&x)[n]) const { Elem<DTYPE>::unpack(raw, x); }
+  __device__ static __forceinline__ void store(type* p, const float (&x)[n]) {
+    *reinterpret_cast<u32x4_any*>(p) = Elem<DTYPE>::pack(x);
+  }
+};
+template <int DTYPE>
+struct Piece<DTYPE, 1> {
+  typedef typename Elem<DTYPE>::type type;
+  type raw;
+  __device__ __forceinline__ void load(const type* p) { raw = *p; }
+  __device__ __forceinline__ void unpack(float (&x)[1]) const { x[0] = Elem<DTYPE>::up(raw); }
+  __device__ static __forceinline__ void store(type* p, const float (&x)[1]) { *p = Elem<DTYPE>::down(x[0]); }
+};
+
 // kVec elements from x + col; columns past the row's end read as `fill`.
 template <int DTYPE>
 __device__ __forceinline__ void load_vec(const typename Elem<DTYPE>::type* x, int col, int V,
@@ -151,30 +172,37 @@ __device__ __forceinline__ RowStats row_stats_join(const RowStats& a, const RowS
   return r;
 }
 
-// Adds n elements; rate = log2(e) / tau.
+// Adds n elements to a part whose maximum already covers them; rate = log2(e) / tau.
 template <int n>
 __device__ __forceinline__ void row_stats_add(RowStats& a, const float (&x)[n], float rate) {
-  float top = x[0];
 #pragma unroll
-  for (int i = 1; i < n; ++i) top = fmaxf(top, x[i]);
-  const float m = fmaxf(a.m, top);
+  for (int i = 0; i < n; ++i) {
+    const float d = x[i] - a.m;
+    const float e = __builtin_amdgcn_exp2f(d * rate);
+    a.s += e;
+    a.w += e * fmaxf(d, kFarBelow);
+  }
+}
+// Raises the maximum to cover n elements.
+template <int n>
+__device__ __forceinline__ float row_max(float m, const float (&x)[n]) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) m = fmaxf(m, x[i]);
+  return m;
+}
+__device__ __forceinline__ void row_stats_raise(RowStats& a, float m, float rate) {
   const float d = fmaxf(a.m - m, kFarBelow);
   const float f = __builtin_amdgcn_exp2f(d * rate);
   a.w = f * (a.w + a.s * d);
   a.s *= f;
   a.m = m;
-#pragma unroll
-  for (int i = 0; i < n; ++i) {
-    const float di = x[i] - m;
-    const float e = __builtin_amdgcn_exp2f(di * rate);
-    a.s += e;
-    a.w += e * fmaxf(di, kFarBelow);
-  }
 }
 
-__device__ __forceinline__ RowStats row_stats_wave(RowStats a, float rate) {
+// Joins the parts of `lanes` neighbouring lanes (a power of two); each of them gets the result.
+template <int lanes>
+__device__ __forceinline__ RowStats row_stats_lanes(RowStats a, float rate) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
+  for (int d = lanes / 2; d > 0; d >>= 1) {
     const RowStats o = {__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64), __shfl_xor(a.w, d, 64)};
     a = row_stats_join(a, o, rate);
   }
@@ -184,24 +212,151 @@ __device__ __forceinline__ RowStats row_stats_wave(RowStats a, float rate) {
 // Over a workgroup of WAVES waves; every thread gets the result.  s_part: WAVES entries of LDS.
 template <int WAVES>
 __device__ __forceinline__ RowStats row_stats_block(RowStats a, float rate, RowStats* s_part) {
-  a = row_stats_wave(a, rate);
+  a = row_stats_lanes<64>(a, rate);
   if constexpr (WAVES > 1) {
     if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = s_part[0];
-#pragma unroll
-    for (int i = 1; i < WAVES; ++i) a = row_stats_join(a, s_part[i], rate);
+    a = row_stats_lanes<WAVES>(s_part[threadIdx.x & (WAVES - 1)], rate);
   }
   return a;
 }
 
+// A row in the hands of a workgroup of WAVES waves: pieces of kVec elements, thread t holding the
+// pieces t, t + threads, ..., and the V % kVec elements behind the last whole piece one each.
+// NV > 0: up to NV pieces a thread, which stay in registers, so that the row is read once
+// however often it is looked at; NV = 0: any length, read again each time.
+template <int DTYPE, int WAVES, int NV>
+struct Row {
+  typedef Elem<DTYPE> E;
+  typedef typename E::type type;
+  static constexpr int kThreads = WAVES * 64;
+  static constexpr int kBatch = 4;      // loads in flight of a row that is not held
+  static constexpr uint32_t kNothing = DTYPE == ICAP_DTYPE_F32    ? 0xff800000u
+                                       : DTYPE == ICAP_DTYPE_BF16 ? 0xff80ff80u
+                                                                  : 0xfc00fc00u;      // -inf
+  const type* x;
+  int V, pieces;
+  u32x4 raw[NV > 0 ? NV : 1];
+  float tail;      // -inf without one
+
+  __device__ __forceinline__ u32x4 read(int i) const {
+    // (a thread without an i-th piece reads the last one and forgets it: no branch round a load)
+    u32x4 r = *reinterpret_cast<const u32x4_any*>(x + (size_t)min(i, pieces - 1) * E::kVec);
+    if (i >= pieces) r = u32x4{kNothing, kNothing, kNothing, kNothing};
+    return r;
+  }
+  __device__ __forceinline__ int tail_col() const { return pieces * E::kVec + (int)threadIdx.x; }
+
+  __device__ __forceinline__ void open(const type* row, int n) {
+    x = row;
+    V = n;
+    pieces = n / E::kVec;
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (j * kThreads < pieces) raw[j] = read(j * kThreads + threadIdx.x);
+    }
+    tail = tail_col() < n ? E::up(x[tail_col()]) : -INFINITY;
+  }
+
+  // f(values, first column) for each of this thread's pieces, then for its single element; columns
+  // past the row's end are -inf
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (j * kThreads < pieces) {
+          float v[E::kVec];
+          E::unpack(raw[j], v);
+          f(v, (j * kThreads + (int)threadIdx.x) * E::kVec);
+        }
+    } else {
+      for (int i0 = 0; i0 < pieces; i0 += kBatch * kThreads) {
+        u32x4 r[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) r[j] = read(i0 + j * kThreads + threadIdx.x);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          float v[E::kVec];
+          E::unpack(r[j], v);
+          f(v, (i0 + j * kThreads + (int)threadIdx.x) * E::kVec);
+        }
+      }
+    }
+    const float v[1] = {tail};
+    f(v, tail_col());
+  }
+
+  // This thread's part of the statistics, its maximum among them
+  __device__ __forceinline__ RowStats stats(float rate) const {
+    RowStats a = row_stats_empty();
+    if constexpr (NV > 0) {
+      each([&](const auto& v, int) { a.m = row_max(a.m, v); });
+      each([&](const auto& v, int) { row_stats_add(a, v, rate); });
+    } else {
+      for (int i0 = 0; i0 < pieces; i0 += kBatch * kThreads) {
+        u32x4 r[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) r[j] = read(i0 + j * kThreads + threadIdx.x);
+        float m = a.m;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          float v[E::kVec];
+          E::unpack(r[j], v);
+          m = row_max(m, v);
+        }
+        row_stats_raise(a, m, rate);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          float v[E::kVec];
+          E::unpack(r[j], v);
+          row_stats_add(a, v, rate);
+        }
+      }
+      const float v[1] = {tail};
+      row_stats_raise(a, row_max(a.m, v), rate);
+      row_stats_add(a, v, rate);
+    }
+    return a;
+  }
+
+  // out[column] = f(value, column) in the row's type; out may be the row itself once it was opened
+  // (each thread writes what it alone read)
+  template <class F>
+  __device__ __forceinline__ void write(type* out, F f) const {
+    each([&](const auto& v, int c) {
+      constexpr int n = sizeof(v) / sizeof(float);
+      if (c + n > V) return;
+      float g[n];
+#pragma unroll
+      for (int e = 0; e < n; ++e) g[e] = f(v[e], c + e);
+      Piece<DTYPE, n>::store(out + c, g);
+    });
+  }
+};
+
+// Zeros in a row of V elements.
+template <int DTYPE, int WAVES>
+__device__ __forceinline__ void write_zeros(typename Elem<DTYPE>::type* out, int V) {
+  constexpr int n = Elem<DTYPE>::kVec;
+  const float zero[n] = {}, one[1] = {};
+  for (int i = threadIdx.x; i < V / n; i += WAVES * 64) Piece<DTYPE, n>::store(out + (size_t)i * n, zero);
+  const int c = V / n * n + (int)threadIdx.x;
+  if (c < V) Piece<DTYPE, 1>::store(out + c, one);
+}
+
 // Order of the alternatives: by value, then by the lower column; -0 and +0 are equal, and a NaN
 // counts as -inf.  A larger key is a better alternative and no two columns share one.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint((v == v ? v : -INFINITY) + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float order_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
 __device__ __forceinline__ unsigned long long rank_key(float v, int col) {
-  const float z = v == v ? v + 0.f : -INFINITY;
-  const uint32_t u = __float_as_uint(z);
-  const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)k << 32) | (0xffffffffu - (uint32_t)col);
+  return ((unsigned long long)order_of(v) << 32) | (0xffffffffu - (uint32_t)col);
 }
 __device__ __forceinline__ int rank_col(unsigned long long key) {
   return (int)(0xffffffffu - (uint32_t)key);
