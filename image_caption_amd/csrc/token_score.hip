@@ -51,16 +51,17 @@ __device__ __forceinline__ void top_columns(const Row<DTYPE, WAVES, NV>& row, fl
   } else {
     __syncthreads();
   }
-  // the k-th largest of 64, bit by bit, until exactly k reach the bound
+  // the k-th largest of 64, bit by bit, until exactly k reach the bound or it is known to 12 bits
+  // of the mantissa (a bound a little too low lets few more elements in)
   const uint32_t mine = order_of(group);
   uint32_t bound = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= 12; --bit) {
     const uint32_t next = bound | (1u << bit);
     const int reach = __popcll(__ballot(mine >= next));
     if (reach >= k) bound = next;
     if (reach == k) break;
   }
-  const float least = order_value(bound);
+  const float least = fmaxf(order_value(bound), kLowest);
   if (top >= least)
     row.each([&](const auto& v, int c) {
       if (row_max(-INFINITY, v) < least) return;
@@ -136,22 +137,18 @@ __global__ __launch_bounds__(WAVES * 64) void token_log_probs_kernel(ScoreArgs p
   data.open(x, p.V);
   const bool inside = token >= 0 && token < p.V;
   const float x_t = inside ? E::up(x[token]) : NAN;
-  const RowStats part = data.stats(kLog2e);
-  const RowStats a = row_stats_block<WAVES>(part, kLog2e, s_part);
-  const bool none = a.s == 0.f;                 // every logit is -inf
-  const float m = none ? -INFINITY : a.m;
-  const float log_s = none ? 0.f : logf(a.s);
+  const auto r = data.result(kLog2e, s_part);
   if (tid == 0) {
-    p.log_probs[row] = inside && none ? -INFINITY : (x_t - m) - log_s;
-    p.entropy[row] = none ? 0.f : log_s - a.w / a.s;
-    p.stats[2 * (size_t)row] = m;
-    p.stats[2 * (size_t)row + 1] = log_s;
+    p.log_probs[row] = inside && r.none ? -INFINITY : (x_t - r.m) - r.log_s;
+    p.entropy[row] = r.entropy;
+    p.stats[2 * (size_t)row] = r.m;
+    p.stats[2 * (size_t)row + 1] = r.log_s;
   }
   if (p.k == 0) return;
-  top_columns(data, part.m, p.k, s_top, [&](int rank, unsigned long long key) {
+  top_columns(data, r.top, p.k, s_top, [&](int rank, unsigned long long key) {
     const int col = rank_col(key);
     p.top_ids[(size_t)row * p.k + rank] = col;
-    p.top_log_probs[(size_t)row * p.k + rank] = none ? -INFINITY : (E::up(x[col]) - m) - log_s;
+    p.top_log_probs[(size_t)row * p.k + rank] = r.none ? -INFINITY : (E::up(x[col]) - r.m) - r.log_s;
   });
 }
 
@@ -296,21 +293,20 @@ __global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p)
   }
   Row<DTYPE, WAVES, NV> data;
   data.open(x, p.V);
-  const RowStats a = row_stats_block<WAVES>(data.stats(rate), rate, s_part);
-  const bool none = a.s == 0.f;
-  const float log_s = logf(a.s), inv_s = 1.f / a.s;
+  const auto a = data.result(rate, s_part);
+  const float inv_s = __builtin_amdgcn_exp2f(-a.log_s * kLog2e);
   if (tid < 64) {
     float sum = 0.f;
     for (int k = tid; k < p.K; k += 64) {
       const float q = s_q[k];
-      const float lp = none ? -INFINITY : (s_x[k] - a.m) * inv_tau - log_s;
+      const float lp = a.none ? -INFINITY : (s_x[k] - a.m) * inv_tau - a.log_s;
       if (s_id[k] >= 0 && !(q == 0.f)) sum += q * (s_log_q[k] - lp);
     }
     sum = wave_sum(sum) * p.tau * p.tau;
     if (tid == 0) p.loss[row] = s_bad ? NAN : sum;
   }
   if (!g) return;
-  if (coef == 0.f || (none && !s_bad)) {
+  if (coef == 0.f || (a.none && !s_bad)) {
     write_zeros<DTYPE, WAVES>(g, p.V);
     return;
   }

@@ -19,8 +19,8 @@ struct RowView {
 
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
-// A difference to the row maximum is held at this: -inf and the lowest float are at -1e30 all the
-// same a weight of exactly 0, and 0 * -1e30 stays 0 where 0 * -inf would not.
+// A difference to the row's reference is held at this: -inf and the lowest float have at -1e30 all
+// the same a weight of exactly 0, and 0 * -1e30 stays 0 where 0 * -inf would not.
 constexpr float kFarBelow = -1e30f;
 
 #if defined(__HIPCC__)
@@ -150,52 +150,64 @@ __device__ __forceinline__ void store_vec(typename Elem<DTYPE>::type* x, int col
   }
 }
 
-// Running statistics of a soft-max over part of a row, all relative to the maximum m so far:
-// s = sum exp((x - m) / tau), w = sum exp((x - m) / tau) * (x - m).  Parts join in any tree of
-// a fixed shape, so a row's result does not depend on timing.
-//   log-sum-exp = m / tau + ln s,   entropy = ln s - w / (tau s)
-// m starts at the lowest float instead of -inf, so that x - m is defined for a part of -inf
-// alone (its s stays 0).  A NaN, and the inf - inf of an infinite maximum, end in s and stay.
+// Statistics of a soft-max over part of a row, in powers of two: with rate = log2(e) / tau and a
+// reference c near rate * m, m the maximum so far,
+//   y = rate * x - c (one fused multiply-add),   s = sum 2^y,   w = sum 2^y y.
+// c is rate * m rounded; it is the same number for every element, so its rounding cancels.
+//   log2 of the sum = c + log2 s,   entropy = ln 2 (log2 s - w / s)
+// Parts join in a tree of a fixed shape, so a row's result does not depend on timing.  m starts at
+// the lowest float instead of -inf, so that a part of -inf alone has s = 0 and no NaN.  A NaN, and
+// the inf - inf of an infinite maximum, end in s and stay.
 struct RowStats {
   float m, s, w;
 };
+constexpr float kLowest = -3.4028234663852886e38f;
 
-__device__ __forceinline__ RowStats row_stats_empty() { return {-3.4028234663852886e38f, 0.f, 0.f}; }
+__device__ __forceinline__ RowStats row_stats_empty() { return {kLowest, 0.f, 0.f}; }
 
-__device__ __forceinline__ RowStats row_stats_join(const RowStats& a, const RowStats& b, float rate) {
-  RowStats r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = fmaxf(a.m - r.m, kFarBelow), db = fmaxf(b.m - r.m, kFarBelow);
-  const float fa = __builtin_amdgcn_exp2f(da * rate), fb = __builtin_amdgcn_exp2f(db * rate);
-  r.s = a.s * fa + b.s * fb;
-  r.w = fa * (a.w + a.s * da) + fb * (b.w + b.s * db);
-  return r;
+// Held within +-2^24, where the rounding of rate * m is at most one: a part further below has
+// y <= 0 and next to no weight beside any other, and a row whose own maximum is further out is summed
+// another way (Row::stats_far).
+constexpr float kRefLimit = 16777216.f;
+__device__ __forceinline__ float row_ref(float m, float rate) {
+  return fminf(fmaxf(m * rate, -kRefLimit), kRefLimit);
 }
 
-// Adds n elements to a part whose maximum already covers them; rate = log2(e) / tau.
-template <int n>
-__device__ __forceinline__ void row_stats_add(RowStats& a, const float (&x)[n], float rate) {
+// A sum of products 2^y y with -inf among the y comes out as NaN; `safe` holds y at kFarBelow, which
+// costs one instruction of eight and so is left out where a look at the result tells.
+template <bool safe, int n>
+__device__ __forceinline__ void row_stats_add(float& s, float& w, const float (&x)[n], float rate, float c) {
 #pragma unroll
   for (int i = 0; i < n; ++i) {
-    const float d = x[i] - a.m;
-    const float e = __builtin_amdgcn_exp2f(d * rate);
-    a.s += e;
-    a.w += e * fmaxf(d, kFarBelow);
+    const float y = __builtin_fmaf(x[i], rate, -c);
+    const float e = __builtin_amdgcn_exp2f(y);
+    s += e;
+    w = __builtin_fmaf(e, safe ? fmaxf(y, kFarBelow) : y, w);
   }
 }
-// Raises the maximum to cover n elements.
 template <int n>
 __device__ __forceinline__ float row_max(float m, const float (&x)[n]) {
 #pragma unroll
   for (int i = 0; i < n; ++i) m = fmaxf(m, x[i]);
   return m;
 }
-__device__ __forceinline__ void row_stats_raise(RowStats& a, float m, float rate) {
-  const float d = fmaxf(a.m - m, kFarBelow);
-  const float f = __builtin_amdgcn_exp2f(d * rate);
-  a.w = f * (a.w + a.s * d);
-  a.s *= f;
-  a.m = m;
+// Takes sums from reference a to reference b.  (No contraction here and in the join: a product
+// fused into one side's addition would make the join of a and b differ from that of b and a, and the
+// lanes of a butterfly end with different last bits.)
+__device__ __forceinline__ void row_stats_move(float& s, float& w, float a, float b) {
+#pragma clang fp contract(off)
+  const float d = fmaxf(a - b, kFarBelow);
+  const float f = __builtin_amdgcn_exp2f(d);
+  w = f * (w + s * d);
+  s *= f;
+}
+
+__device__ __forceinline__ RowStats row_stats_join(RowStats a, RowStats b, float rate) {
+#pragma clang fp contract(off)
+  const float m = fmaxf(a.m, b.m), c = row_ref(m, rate);
+  row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
+  row_stats_move(b.s, b.w, row_ref(b.m, rate), c);
+  return {m, a.s + b.s, a.w + b.w};
 }
 
 // Joins the parts of `lanes` neighbouring lanes (a power of two); each of them gets the result.
@@ -288,12 +300,34 @@ struct Row {
     f(v, tail_col());
   }
 
-  // This thread's part of the statistics, its maximum among them
+  // This thread's part of the statistics
   __device__ __forceinline__ RowStats stats(float rate) const {
     RowStats a = row_stats_empty();
     if constexpr (NV > 0) {
       each([&](const auto& v, int) { a.m = row_max(a.m, v); });
-      each([&](const auto& v, int) { row_stats_add(a, v, rate); });
+      const float c = row_ref(a.m, rate);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (j * kThreads < pieces) {
+          float v[E::kVec];
+          E::unpack(raw[j], v);
+          if ((j + 1) * kThreads <= pieces) row_stats_add<false>(a.s, a.w, v, rate, c);
+          else row_stats_add<true>(a.s, a.w, v, rate, c);
+        }
+      }
+      if (!(a.w == a.w)) {
+        a.s = a.w = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if (j * kThreads < pieces) {
+            float v[E::kVec];
+            E::unpack(raw[j], v);
+            row_stats_add<true>(a.s, a.w, v, rate, c);
+          }
+        }
+      }
+      const float v[1] = {tail};
+      row_stats_add<true>(a.s, a.w, v, rate, c);
     } else {
       for (int i0 = 0; i0 < pieces; i0 += kBatch * kThreads) {
         u32x4 r[kBatch];
@@ -306,19 +340,82 @@ struct Row {
           E::unpack(r[j], v);
           m = row_max(m, v);
         }
-        row_stats_raise(a, m, rate);
+        const float c = row_ref(m, rate);
+        row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
+        a.m = m;
+        const float s = a.s, w = a.w;
+        // (unpacked again below: held unpacked they would cost 32 registers and half the waves)
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          float v[E::kVec];
-          E::unpack(r[j], v);
-          row_stats_add(a, v, rate);
+        for (int j = 0; j < kBatch; ++j) asm volatile("" : "+v"(r[j]));
+        const bool whole = i0 + kBatch * kThreads <= pieces;
+        if (whole) {
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            float v[E::kVec];
+            E::unpack(r[j], v);
+            row_stats_add<false>(a.s, a.w, v, rate, c);
+          }
+        }
+        if (!whole || !(a.w == a.w)) {
+          a.s = s;
+          a.w = w;
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            float v[E::kVec];
+            E::unpack(r[j], v);
+            row_stats_add<true>(a.s, a.w, v, rate, c);
+          }
         }
       }
       const float v[1] = {tail};
-      row_stats_raise(a, row_max(a.m, v), rate);
-      row_stats_add(a, v, rate);
+      const float m = row_max(a.m, v), c = row_ref(m, rate);
+      row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
+      a.m = m;
+      row_stats_add<true>(a.s, a.w, v, rate, c);
     }
     return a;
+  }
+
+  // The same for a row whose maximum m is known and so large that rate * x would overflow or round
+  // off what tells the elements apart: y = rate (x - m).
+  __device__ __forceinline__ RowStats stats_far(float m, float rate) const {
+    RowStats a = {m, 0.f, 0.f};
+    const float big = m;
+    for (int i = threadIdx.x; i < V; i += kThreads) {
+      const float y = (E::up(x[i]) - big) * rate;
+      const float e = __builtin_amdgcn_exp2f(y);
+      a.s += e;
+      a.w = __builtin_fmaf(e, fmaxf(y, kFarBelow), a.w);
+    }
+    return a;
+  }
+
+  // The row's statistics, the same in every thread.  top: this thread's own maximum.
+  struct Result {
+    float top;        // this thread's own maximum
+    float m;          // the row's
+    float log_s;      // ln sum exp((x - m) / tau)
+    float entropy;
+    bool none;        // every element is -inf
+  };
+  __device__ __forceinline__ Result result(float rate, RowStats* s_part) const {
+    const RowStats part = stats(rate);
+    RowStats a = row_stats_block<WAVES>(part, rate, s_part);
+    const float c = row_ref(a.m, rate);
+    float off = __builtin_fmaf(a.m, rate, -c);      // of the reference from the maximum
+    if (!(fabsf(c) < kRefLimit)) {
+      // (the joins of parts with one maximum only add)
+      if constexpr (WAVES > 1) __syncthreads();
+      a = row_stats_block<WAVES>(stats_far(a.m, rate), rate, s_part);
+      off = 0.f;
+    }
+    Result r;
+    r.top = part.m;
+    r.none = a.s == 0.f;
+    r.m = r.none ? -INFINITY : a.m;
+    r.log_s = r.none ? 0.f : logf(a.s) - off * kLn2;
+    r.entropy = r.none ? 0.f : logf(a.s) - kLn2 * (a.w / a.s);
+    return r;
   }
 
   // out[column] = f(value, column) in the row's type; out may be the row itself once it was opened

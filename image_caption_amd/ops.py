@@ -37,7 +37,9 @@ def current_stream():
         devs.clear()
         _tls.frame = None
     _tls.dev = dev
-    return torch.cuda.current_stream(dev).cuda_stream
+    # (the handle behind torch.cuda.current_stream(dev).cuda_stream, without the 2 us of making that
+    # object: a fifth of a small call)
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _call(name, *args):

@@ -237,6 +237,19 @@ def test_gradients_in_place_and_into_views(kind, V):
     assert torch.equal(buf[:, :5], keep[:, :5]) and torch.equal(buf[:, V + 5:], keep[:, V + 5:])
 
 
+@pytest.mark.parametrize("N,V", [(600, 1001), (600, 9000), (40, 9000), (7, 70001), (40, 50000)])
+def test_the_same_call_gives_the_same_bits(N, V):
+    """Every thread of a workgroup that writes a result has to hold the same statistics."""
+    from image_caption_amd import ops
+    rng = np.random.default_rng(N)
+    x, tokens = _logits(rng, N, V, "bf16"), _ids(rng.integers(0, V, N))
+    ti, tl, g = _ids(rng.integers(0, V, (N, 70))), _logits(rng, N, 70, "f32"), _dev(rng.standard_normal(N))
+    first = ops.token_log_probs(x, tokens, top_k=32) + ops.distill_loss(x, tl, ti, 2.0, g)
+    for _ in range(8):
+        again = ops.token_log_probs(x, tokens, top_k=32) + ops.distill_loss(x, tl, ti, 2.0, g)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 def test_offsets_past_32_bits():
     """Rows that start 2^31 elements and more behind the first."""
     from image_caption_amd import ops
