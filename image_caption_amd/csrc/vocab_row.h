@@ -233,6 +233,39 @@ __device__ __forceinline__ RowStats row_stats_block(RowStats a, float rate, RowS
   return a;
 }
 
+// One element of a row whose maximum m is known and so large that rate * x would overflow or round off
+// what tells the elements apart: y = rate (x - m).
+__device__ __forceinline__ void row_stats_add_far(RowStats& a, float x, float rate) {
+  const float y = (x - a.m) * rate;
+  const float e = __builtin_amdgcn_exp2f(y);
+  a.s += e;
+  a.w = __builtin_fmaf(e, fmaxf(y, kFarBelow), a.w);
+}
+
+// What a row's joined statistics say; far(m) sums the row again by row_stats_add_far.
+struct RowResult {
+  float m;          // the maximum
+  float log_s;      // ln sum exp((x - m) / tau)
+  float entropy;
+  bool none;        // every element is -inf
+};
+template <class Far>
+__device__ __forceinline__ RowResult row_result(RowStats a, float rate, Far far) {
+  const float c = row_ref(a.m, rate);
+  float off = __builtin_fmaf(a.m, rate, -c);      // of the maximum from the reference
+  if (!(fabsf(c) < kRefLimit)) {
+    a = far(a.m);
+    off = 0.f;
+  }
+  RowResult r;
+  const float log_s = logf(a.s);
+  r.none = a.s == 0.f;
+  r.m = r.none ? -INFINITY : a.m;
+  r.log_s = r.none ? 0.f : log_s - off * kLn2;
+  r.entropy = r.none ? 0.f : log_s - kLn2 * (a.w / a.s);
+  return r;
+}
+
 // A row in the hands of a workgroup of WAVES waves: pieces of kVec elements, thread t holding the
 // pieces t, t + threads, ..., and the V % kVec elements behind the last whole piece one each.
 // NV > 0: up to NV pieces a thread, which stay in registers, so that the row is read once
@@ -376,46 +409,14 @@ struct Row {
     return a;
   }
 
-  // The same for a row whose maximum m is known and so large that rate * x would overflow or round
-  // off what tells the elements apart: y = rate (x - m).
-  __device__ __forceinline__ RowStats stats_far(float m, float rate) const {
-    RowStats a = {m, 0.f, 0.f};
-    const float big = m;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-      const float y = (E::up(x[i]) - big) * rate;
-      const float e = __builtin_amdgcn_exp2f(y);
-      a.s += e;
-      a.w = __builtin_fmaf(e, fmaxf(y, kFarBelow), a.w);
-    }
-    return a;
-  }
-
-  // The row's statistics, the same in every thread.  top: this thread's own maximum.
-  struct Result {
-    float top;        // this thread's own maximum
-    float m;          // the row's
-    float log_s;      // ln sum exp((x - m) / tau)
-    float entropy;
-    bool none;        // every element is -inf
-  };
-  __device__ __forceinline__ Result result(float rate, RowStats* s_part) const {
-    const RowStats part = stats(rate);
-    RowStats a = row_stats_block<WAVES>(part, rate, s_part);
-    const float c = row_ref(a.m, rate);
-    float off = __builtin_fmaf(a.m, rate, -c);      // of the reference from the maximum
-    if (!(fabsf(c) < kRefLimit)) {
-      // (the joins of parts with one maximum only add)
+  // The row's statistics, the same in every thread
+  __device__ __forceinline__ RowResult result(float rate, RowStats* s_part) const {
+    return row_result(row_stats_block<WAVES>(stats(rate), rate, s_part), rate, [&](float m) {
+      RowStats f = {m, 0.f, 0.f};
+      for (int i = threadIdx.x; i < V; i += kThreads) row_stats_add_far(f, E::up(x[i]), rate);
       if constexpr (WAVES > 1) __syncthreads();
-      a = row_stats_block<WAVES>(stats_far(a.m, rate), rate, s_part);
-      off = 0.f;
-    }
-    Result r;
-    r.top = part.m;
-    r.none = a.s == 0.f;
-    r.m = r.none ? -INFINITY : a.m;
-    r.log_s = r.none ? 0.f : logf(a.s) - off * kLn2;
-    r.entropy = r.none ? 0.f : logf(a.s) - kLn2 * (a.w / a.s);
-    return r;
+      return row_stats_block<WAVES>(f, rate, s_part);
+    });
   }
 
   // out[column] = f(value, column) in the row's type; out may be the row itself once it was opened
