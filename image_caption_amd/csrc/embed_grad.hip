@@ -14,7 +14,7 @@ __device__ __forceinline__ int piece_col(int c, int n, int D) { return min(c, D 
 // One group of lanes per token, kLookupAhead tokens at a time.
 constexpr int kLookupAhead = 4;
 
-template <int DTYPE, int n>
+template <int DTYPE, int n, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_scaled_kernel(const void* table, const int32_t* ids,
                                                                void* out, int N, int V, int D, float scale,
                                                                int pad, int lanes) {
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void embedding_scaled_kernel(const void* table
       x[j].unpack(v);
 #pragma unroll
       for (int e = 0; e < n; ++e) v[e] = id[j] < 0 ? 0.f : v[e] * scale;
-      P::store((typename P::type*)out + (size_t)(n0 + j) * D + c, v);
+      P::template store<STREAM>((typename P::type*)out + (size_t)(n0 + j) * D + c, v);
     }
   }
 }
@@ -409,11 +409,14 @@ int icap_embedding_scaled(const void* table, int dtype, const int32_t* ids, void
   if (N == 0) return ICAP_OK;
   const int vec = vec_of(dtype, D), lanes = lanes_of(D, vec);
   const dim3 grid(ceil_div(ceil_div(N, kLookupAhead), 256 / lanes));
-#define LAUNCH(T, n)                                                                            \
-  hipLaunchKernelGGL((embedding_scaled_kernel<T, n>), grid, dim3(256), 0, (hipStream_t)stream, table, \
+  const bool streamed = stream_writes((size_t)N * D * (dtype == ICAP_DTYPE_F32 ? 4 : 2));
+#define LAUNCH_S(T, n, S)                                                                             \
+  hipLaunchKernelGGL((embedding_scaled_kernel<T, n, S>), grid, dim3(256), 0, (hipStream_t)stream, table, \
                      ids, out, N, V, D, scale, pad_token, lanes)
+#define LAUNCH(T, n) do { if (streamed) LAUNCH_S(T, n, true); else LAUNCH_S(T, n, false); } while (0)
   ICAP_BY_TYPE_AND_VEC(dtype, vec, LAUNCH);
 #undef LAUNCH
+#undef LAUNCH_S
   ICAP_LAUNCH_CHECK("embedding_scaled_kernel");
   return ICAP_OK;
 }

@@ -52,11 +52,10 @@ __device__ __forceinline__ float kth_of_lanes(float v, int k) {
 
 // One wave's share of a row: pieces [from, to) of kVec elements, read once in batches of kBatch a
 // lane, and for the row's last wave the elements behind the last whole piece.
-template <int DTYPE>
+template <int DTYPE, bool STREAM>
 struct Share {
   typedef Elem<DTYPE> E;
   typedef typename E::type type;
-  static constexpr uint32_t kNothing = Row<DTYPE, 1, 0>::kNothing;
   static constexpr int kBatch = kBatchElems / E::kVec;
   const type* x;
   int from, to, lane;
@@ -65,8 +64,8 @@ struct Share {
 
   __device__ __forceinline__ int piece(int b, int j) const { return from + (b * kBatch + j) * 64 + lane; }
   __device__ __forceinline__ u32x4 read(int i) const {
-    u32x4 r = *reinterpret_cast<const u32x4_any*>(x + (size_t)min(i, to - 1) * E::kVec);
-    if (i >= to) r = u32x4{kNothing, kNothing, kNothing, kNothing};
+    u32x4 r = load16<STREAM>(x + (size_t)min(i, to - 1) * E::kVec);
+    if (i >= to) r = u32x4{E::kNothing, E::kNothing, E::kNothing, E::kNothing};
     return r;
   }
 };
@@ -75,11 +74,11 @@ struct Share {
 // left).  While the share is read the wave keeps a bound that at least k elements have reached - the
 // k-th largest of the lanes' maxima so far, renewed after 1, 2, 4, 8 ... batches - and notes the
 // batches of a lane that reach it; in the end some k to 2k of them are read again.
-template <int DTYPE, bool TOP>
-__device__ __forceinline__ RowStats share_scan(const Share<DTYPE>& sh, float rate, int k, TopScratch& s,
+template <int DTYPE, bool TOP, bool STREAM>
+__device__ __forceinline__ RowStats share_scan(const Share<DTYPE, STREAM>& sh, float rate, int k, TopScratch& s,
                                                unsigned long long* best) {
   typedef Elem<DTYPE> E;
-  constexpr int kBatch = Share<DTYPE>::kBatch;
+  constexpr int kBatch = Share<DTYPE, STREAM>::kBatch;
   const unsigned long long lower = (1ull << sh.lane) - 1;
   RowStats a = row_stats_empty();
   const int batches = (sh.to - sh.from + kBatch * 64 - 1) / (kBatch * 64);
@@ -139,7 +138,7 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE>& sh, float rat
     row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
     a.m = m;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) row_stats_add<true>(a.s, a.w, v[j], rate, c);
+    for (int j = 0; j < kBatch; ++j) row_stats_add(a.s, a.w, v[j], rate, c);
     if constexpr (TOP) {
       if (b == renew) {
         bound = kth_of_lanes(a.m, k);
@@ -152,7 +151,7 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE>& sh, float rat
   const float m = row_max(a.m, tail), c = row_ref(m, rate);
   row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
   a.m = m;
-  row_stats_add<true>(a.s, a.w, tail, rate, c);
+  row_stats_add(a.s, a.w, tail, rate, c);
   if constexpr (TOP) {
     if (__any(sh.tail_col >= 0)) note(sh.tail_col >= 0 ? sh.tail : -INFINITY, -1 - sh.tail_col);
     squeeze();
@@ -212,7 +211,7 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE>& sh, float rat
 // P waves to a row, 4 / P rows to a workgroup (P = 1, 2) or one (P = 4, 8).  The waves of a row
 // meet once, when each has its share's statistics and its k best columns in LDS; the first joins
 // them.  Rows alone in a wave wait for nobody.
-template <int DTYPE, int P, bool TOP>
+template <int DTYPE, int P, bool TOP, bool STREAM>
 __global__ __launch_bounds__((P < 4 ? 4 : P) * 64, 8) void token_log_probs_kernel(ScoreArgs p) {
   typedef Elem<DTYPE> E;
   constexpr int WAVES = P < 4 ? 4 : P;
@@ -231,7 +230,7 @@ __global__ __launch_bounds__((P < 4 ? 4 : P) * 64, 8) void token_log_probs_kerne
     const int pieces = p.V / E::kVec;
     // shares of whole batches
     const int each = ((pieces + P - 1) / P + 63) / 64 * 64;
-    Share<DTYPE> sh;
+    Share<DTYPE, STREAM> sh;
     sh.x = x;
     sh.from = min(pieces, part * each);
     sh.to = min(pieces, sh.from + each);
@@ -239,7 +238,7 @@ __global__ __launch_bounds__((P < 4 ? 4 : P) * 64, 8) void token_log_probs_kerne
     const int tail_col = pieces * E::kVec + lane;
     sh.tail_col = part == P - 1 && tail_col < p.V ? tail_col : -1;
     sh.tail = sh.tail_col >= 0 ? E::up(x[tail_col]) : -INFINITY;
-    a = row_stats_lanes<64>(share_scan<DTYPE, TOP>(sh, kLog2e, p.k, s_top[TOP ? wave : 0], s_best[TOP ? wave : 0]), kLog2e);
+    a = row_stats_lanes<64>(share_scan<DTYPE, TOP, STREAM>(sh, kLog2e, p.k, s_top[TOP ? wave : 0], s_best[TOP ? wave : 0]), kLog2e);
   }
   if constexpr (P > 1) {
     if (lane == 0) s_part[wave] = a;
@@ -314,7 +313,7 @@ struct ScoreGradArgs {
 // Element by element, so a row is cut into shares of kGradPieces pieces a thread.
 constexpr int kGradPieces = 4;
 
-template <int DTYPE>
+template <int DTYPE, bool STREAM>
 __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs p) {
   typedef Elem<DTYPE> E;
   typedef typename E::type type;
@@ -332,7 +331,8 @@ __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs 
     const float zero[E::kVec] = {};
 #pragma unroll
     for (int j = 0; j < kGradPieces; ++j)
-      if (first + j * NT < pieces) Piece<DTYPE, E::kVec>::store(g + (size_t)(first + j * NT) * E::kVec, zero);
+      if (first + j * NT < pieces) 
+        Piece<DTYPE, E::kVec>::template store<STREAM>(g + (size_t)(first + j * NT) * E::kVec, zero);
     if (has_tail) g[tail] = E::down(0.f);
     return;
   }
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs 
 #pragma unroll
   for (int j = 0; j < kGradPieces; ++j)
     if (pieces > 0)
-      raw[j] = *reinterpret_cast<const u32x4_any*>(x + (size_t)min(first + j * NT, pieces - 1) * E::kVec);
+      raw[j] = load16<STREAM>(x + (size_t)min(first + j * NT, pieces - 1) * E::kVec);
 #pragma unroll
   for (int j = 0; j < kGradPieces; ++j) {
     const int i = first + j * NT;
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs 
     E::unpack(raw[j], v);
 #pragma unroll
     for (int e = 0; e < E::kVec; ++e) v[e] = grad(v[e], i * E::kVec + e);
-    Piece<DTYPE, E::kVec>::store(g + (size_t)i * E::kVec, v);
+    Piece<DTYPE, E::kVec>::template store<STREAM>(g + (size_t)i * E::kVec, v);
   }
   if (has_tail) g[tail] = E::down(grad(t, tail));
 }
@@ -386,93 +386,126 @@ __device__ __forceinline__ float load_typed(const void* p, int dtype, size_t i) 
   return (float)((const _Float16*)p)[i];
 }
 
+// Only what goes through LDS is ordered: loads and stores of device memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // loss = tau^2 sum_k q_k (log q_k - log p[id_k]),  q = soft-max of the teacher's K logits at tau,
 // p = soft-max of the row at tau;   d loss / d x_j = tau (p_j - sum over k with id_k = j of q_k)
-template <int DTYPE, int WAVES, int NV>
+//
+// A workgroup reads a row into registers, sums it, and writes the gradient from there; the row is
+// read while the first wave takes the teacher's entries along, and one barrier hands their q and
+// the waves' sums round.  (A workgroup that goes through several rows and reads the next one into a
+// second set of registers was slower, 158 against 122 us for 2560 rows of 50000 in bf16: the
+// registers cost it half of its neighbours, which hide the same latency.)
+template <int DTYPE, int WAVES, int NV, bool STREAM>
 __global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p) {
   typedef Elem<DTYPE> E;
+  typedef typename E::type type;
   __shared__ RowStats s_part[WAVES];
   __shared__ int s_id[kMaxTeacher];
   __shared__ float s_q[kMaxTeacher], s_log_q[kMaxTeacher], s_x[kMaxTeacher];
-  __shared__ int s_alive, s_bad;
-  const int row = blockIdx.y * gridDim.x + blockIdx.x, tid = threadIdx.x;
+  __shared__ int s_state;                    // 1: entries there, 2: an id outside the vocabulary
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.y * gridDim.x + blockIdx.x;
   if (row >= p.N) return;
-  const typename E::type* x = (const typename E::type*)p.logits + p.view.at(row);
-  typename E::type* g = p.out ? (typename E::type*)p.out + p.out_view.at(row) : nullptr;
   const float inv_tau = 1.f / p.tau, rate = kLog2e * inv_tau;
-  if (tid < 64) {
+  type* g = p.out ? (type*)p.out + p.out_view.at(row) : nullptr;
+  // every wave looks for itself whether the teacher has an entry
+  bool any = false;
+  for (int k = lane; k < p.K; k += 64) any |= p.t_ids[(size_t)row * p.K + k] != -1;
+  if (!__any(any)) {
+    if (tid == 0) p.loss[row] = 0.f;
+    if (g) write_zeros<DTYPE, WAVES, STREAM>(g, p.V);
+    return;
+  }
+  Row<DTYPE, WAVES, NV, STREAM> data;
+  data.open((const type*)p.logits + p.view.at(row), p.V);
+  const float coef = g ? p.g_loss[row] * p.tau : 0.f;
+  if (wave == 0) {      // (a lane reads back only what it wrote itself)
+    bool bad = false, entries = false;
     float top = -INFINITY;
-    bool alive = false, bad = false;
-    for (int k = tid; k < p.K; k += 64) {
+#pragma unroll 1
+    for (int k = lane; k < p.K; k += 64) {
       const int id = p.t_ids[(size_t)row * p.K + k];
-      const bool in = id >= 0 && id < p.V;
+      const bool in = (unsigned)id < (unsigned)p.V;
       const float t = id == -1 ? -INFINITY : load_typed(p.t_logits, p.t_dtype, (size_t)row * p.K + k);
       bad |= id != -1 && !in;
-      alive |= !(t == -INFINITY);
-      s_id[k] = in ? id : -1;
-      s_log_q[k] = t;
-      s_x[k] = in ? E::up(x[id]) : 0.f;
+      entries |= !(t == -INFINITY);
       top = fmaxf(top, t);
+      s_id[k] = in ? id : -1;
+      s_x[k] = in ? E::up(data.x[id]) : 0.f;
+      s_log_q[k] = t;
     }
-    alive = __any(alive);
     bad = __any(bad);
+    entries = __any(entries);
     top = wave_max(top);
     float sum = 0.f;
-    for (int k = tid; k < p.K; k += 64) {
-      const float e = s_log_q[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((s_log_q[k] - top) * rate);
-      s_q[k] = e;
-      sum += e;
+#pragma unroll 1
+    for (int k = lane; k < p.K; k += 64) {
+      const float t = s_log_q[k];
+      const float q = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((t - top) * rate);
+      s_q[k] = q;
+      sum += q;
     }
     sum = wave_sum(sum);
-    const float log_sum = logf(sum);
-    for (int k = tid; k < p.K; k += 64) {
+    const float log_sum = logf(sum), inv = 1.f / sum;
+#pragma unroll 1
+    for (int k = lane; k < p.K; k += 64) {
       s_log_q[k] = (s_log_q[k] - top) * inv_tau - log_sum;
-      s_q[k] /= sum;
+      s_q[k] *= inv;
     }
-    if (tid == 0) { s_alive = alive; s_bad = bad; }
+    if (lane == 0) s_state = (entries ? 1 : 0) | (bad ? 2 : 0);
   }
-  __syncthreads();
-  const float coef = p.g_loss ? p.g_loss[row] * p.tau : 0.f;
-  if (!s_alive && !s_bad) {
-    if (tid == 0) p.loss[row] = 0.f;
-    if (g) write_zeros<DTYPE, WAVES>(g, p.V);
-    return;
-  }
-  Row<DTYPE, WAVES, NV> data;
-  data.open(x, p.V);
-  const auto a = data.result(rate, s_part);
-  const float inv_s = __builtin_amdgcn_exp2f(-a.log_s * kLog2e);
-  if (tid < 64) {
+  RowStats part = row_stats_lanes<64>(data.sums(rate), rate);
+  if (lane == 0) s_part[wave] = part;
+  lds_barrier();
+  const RowResult r =
+      row_result(row_stats_lanes<WAVES>(s_part[lane & (WAVES - 1)], rate), rate, [&](float m) {
+        RowStats f = {m, 0.f, 0.f};
+        for (int i = tid; i < p.V; i += WAVES * 64) row_stats_add_far(f, E::up(data.x[i]), rate);
+        f = row_stats_lanes<64>(f, rate);
+        __syncthreads();
+        if (lane == 0) s_part[wave] = f;
+        __syncthreads();
+        return row_stats_lanes<WAVES>(s_part[lane & (WAVES - 1)], rate);
+      });
+  const bool bad = s_state & 2, entries = s_state;
+  if (wave == 0) {
     float sum = 0.f;
-    for (int k = tid; k < p.K; k += 64) {
+#pragma unroll 1
+    for (int k = lane; k < p.K; k += 64) {
       const float q = s_q[k];
-      const float lp = a.none ? -INFINITY : (s_x[k] - a.m) * inv_tau - a.log_s;
-      if (s_id[k] >= 0 && !(q == 0.f)) sum += q * (s_log_q[k] - lp);
+      const float lp = r.none ? -INFINITY : (s_x[k] - r.m) * inv_tau - r.log_s;
+      if (!(q == 0.f)) sum += q * (s_log_q[k] - lp);
     }
     sum = wave_sum(sum) * p.tau * p.tau;
-    if (tid == 0) p.loss[row] = s_bad ? NAN : sum;
+    if (lane == 0) p.loss[row] = bad ? NAN : entries ? sum : 0.f;
   }
   if (!g) return;
-  if (coef == 0.f || (a.none && !s_bad)) {
-    write_zeros<DTYPE, WAVES>(g, p.V);
+  if (!entries || coef == 0.f || (r.none && !bad)) {
+    write_zeros<DTYPE, WAVES, STREAM>(g, p.V);
     return;
   }
-  const float c0 = s_bad ? NAN : coef;
-  data.write(g, [&](float v, int) { return c0 * (__builtin_amdgcn_exp2f((v - a.m) * rate) * inv_s); });
-  if (s_bad) return;
-  __syncthreads();
+  const float c0 = bad ? NAN : coef;
+  data.write_softmax(g, r, rate, c0);
+  if (bad) return;
+  __syncthreads();      // the columns' first values are stored
   // the teacher's columns again, the first of several entries with the same id for all of them
+  const float inv_s = __builtin_amdgcn_exp2f(-r.log_s * kLog2e);
   for (int k = tid; k < p.K; k += WAVES * 64) {
     const int id = s_id[k];
     bool first = id >= 0;
-    float q = 0.f;
-    for (int j = 0; j < p.K; ++j)
-      if (s_id[j] == id) {
-        if (j < k) first = false;
-        q += s_q[j];
-      }
-    if (first)
-      g[id] = E::down(c0 * (__builtin_amdgcn_exp2f((s_x[k] - a.m) * rate) * inv_s - q));
+    float sum = 0.f;
+    for (int j = 0; j < p.K; ++j) {
+      const bool same = s_id[j] == id;
+      sum += same ? s_q[j] : 0.f;
+      if (same && j < k) first = false;
+    }
+    if (first) g[id] = E::down(c0 * (__builtin_amdgcn_exp2f((s_x[k] - r.m) * rate) * inv_s - sum));
   }
 }
 
@@ -482,6 +515,8 @@ dim3 row_grid(int N) {
   const int x = N < 65536 ? N : 65536;
   return dim3((unsigned)x, (unsigned)ceil_div(N, x));
 }
+
+size_t row_bytes(int dtype, int N, int V) { return (size_t)N * V * (dtype == ICAP_DTYPE_F32 ? 4 : 2); }
 
 int check_rows(const char* what, int dtype, int N, int V, const RowView& v) {
   ICAP_REQUIRE(dtype == ICAP_DTYPE_F32 || dtype == ICAP_DTYPE_BF16 || dtype == ICAP_DTYPE_F16,
@@ -515,9 +550,13 @@ int waves_per_row(int dtype, int N, int V) {
   return P;
 }
 
-// Waves for a row and pieces a thread holds.  A row goes to as few waves as keep it in registers
-// (their joins cost more, the more there are), and to a large workgroup where rows are few and each
-// should be done soon.
+// Waves for a row and pieces a thread holds: as few waves as keep some 10 pieces a thread or less, 16 of
+// them with 7 while two such workgroups fit a compute unit, and longer rows read twice.  Few rows
+// go to large workgroups: their time is that of one row.  Measured, us, with the floor of one read and
+// one write in brackets: 40000 rows of 2000 in fp32 148 (121) by 2 waves of 4, 156 by 1 of 8, 162 by 4
+// of 4; 10240 of 10000 in fp32 165 (155) by 8 of 5, 175 by 4 of 10; in bf16 96 (77) by 4 of 10, 118 by 8
+// of 5; 2560 of 50000 in bf16 121 (97) by 16 of 7 or 8 of 13, 165 by 16 of 13; 2048 of 50000 in fp32
+// 201 (155) read twice, 201 by 16 of 13.
 struct RowShape {
   int waves, held;
 };
@@ -525,22 +564,21 @@ RowShape row_shape(int dtype, int N, int V) {
   const int pieces = V / (dtype == ICAP_DTYPE_F32 ? 4 : 8);
   const bool many = N > 512;      // two rows a compute unit
   if (pieces <= 64 * (many ? 4 : 1)) return {1, 4};
+  if (many && pieces <= 128 * 4) return {2, 4};
   if (pieces <= 256 * (many ? 4 : 2)) return {4, 4};
-  if (many && pieces <= 256 * 10) return {4, 10};
-  if (pieces <= 1024 * 4) return {16, 4};
-  if (pieces <= 1024 * 8) return {16, 8};
-  if (pieces <= 1024 * 16) return {16, 16};
+  if (many && pieces <= 512 * 5) return dtype == ICAP_DTYPE_F32 ? RowShape{8, 5} : RowShape{4, 10};
+  if (pieces <= 1024 * 7) return {16, 7};
   return {16, 0};
 }
 
-#define ICAP_BY_SHAPE(D, shape, call)                                              \
-  do {                                                                             \
-    if ((shape).waves == 1) call(D, 1, 4);                                         \
+#define ICAP_BY_SHAPE(D, shape, call)              \
+  do {                                             \
+    if ((shape).waves == 1) call(D, 1, 4);         \
+    else if ((shape).waves == 2) call(D, 2, 4);    \
     else if ((shape).waves == 4) { if ((shape).held == 4) call(D, 4, 4); else call(D, 4, 10); } \
-    else if ((shape).held == 4) call(D, 16, 4);                                    \
-    else if ((shape).held == 8) call(D, 16, 8);                                    \
-    else if ((shape).held == 16) call(D, 16, 16);                                  \
-    else call(D, 16, 0);                                                           \
+    else if ((shape).waves == 8) call(D, 8, 5);    \
+    else if ((shape).held == 7) call(D, 16, 7);    \
+    else call(D, 16, 0);                           \
   } while (0)
 #define ICAP_BY_ROWS(dtype, shape, call)                                           \
   do {                                                                             \
@@ -575,12 +613,17 @@ int icap_token_log_probs(const void* logits, int dtype, int N, int V, int rows_i
     return fail(ICAP_ERR_UNSUPPORTED, "token_log_probs: top_k %d is over %d", top_k, ICAP_MAX_ALTERNATIVES);
   ScoreArgs a{logits, view, tokens, N, V, pad_token, top_k, log_probs, entropy, stats, top_ids, top_log_probs};
   const int P = waves_per_row(dtype, N, V);
-#define LAUNCH_P(D, P)                                                                              \
-  do {                                                                                              \
-    const dim3 grid = row_grid(ceil_div(N, P < 4 ? 4 / P : 1)), block((P < 4 ? 4 : P) * 64);         \
-    if (top_k) hipLaunchKernelGGL((token_log_probs_kernel<D, P, true>), grid, block, 0, (hipStream_t)stream, a); \
-    else hipLaunchKernelGGL((token_log_probs_kernel<D, P, false>), grid, block, 0, (hipStream_t)stream, a);      \
+  const dim3 grid = row_grid(ceil_div(N, P < 4 ? 4 / P : 1)), block((P < 4 ? 4 : P) * 64);
+  const bool streamed = stream_reads(row_bytes(dtype, N, V));
+#define LAUNCH_P(D, P)                                                                       \
+  do {                                                                                       \
+    if (top_k && streamed) LAUNCH_4(D, P, true, true);                                       \
+    else if (top_k) LAUNCH_4(D, P, true, false);                                             \
+    else if (streamed) LAUNCH_4(D, P, false, true);                                          \
+    else LAUNCH_4(D, P, false, false);                                                       \
   } while (0)
+#define LAUNCH_4(D, P, TOP, S)                                                               \
+  hipLaunchKernelGGL((token_log_probs_kernel<D, P, TOP, S>), grid, block, 0, (hipStream_t)stream, a)
 #define LAUNCH(D)               \
   do {                          \
     if (P == 1) LAUNCH_P(D, 1);      \
@@ -590,6 +633,7 @@ int icap_token_log_probs(const void* logits, int dtype, int N, int V, int rows_i
   } while (0)
   ICAP_BY_DTYPE(dtype, LAUNCH);
 #undef LAUNCH
+#undef LAUNCH_4
 #undef LAUNCH_P
   ICAP_LAUNCH_CHECK("token_log_probs_kernel");
   return ICAP_OK;
@@ -610,10 +654,14 @@ int icap_token_log_probs_grad(const void* logits, int dtype, int N, int V, int r
   const long long blocks = (long long)N * a.shares;
   if (blocks > kMostBlocks)
     return fail(ICAP_ERR_UNSUPPORTED, "token_log_probs_grad: %d rows of %d are too many for one call", N, V);
-#define LAUNCH(D)                                                                                   \
-  hipLaunchKernelGGL(token_log_probs_grad_kernel<D>, dim3((unsigned)blocks), dim3(NT), 0, (hipStream_t)stream, a)
+  const bool streamed = stream_writes(row_bytes(dtype, N, V));
+#define LAUNCH_S(D, S)                                                                          \
+  hipLaunchKernelGGL((token_log_probs_grad_kernel<D, S>), dim3((unsigned)blocks), dim3(NT), 0,  \
+                     (hipStream_t)stream, a)
+#define LAUNCH(D) do { if (streamed) LAUNCH_S(D, true); else LAUNCH_S(D, false); } while (0)
   ICAP_BY_DTYPE(dtype, LAUNCH);
 #undef LAUNCH
+#undef LAUNCH_S
   ICAP_LAUNCH_CHECK("token_log_probs_grad_kernel");
   return ICAP_OK;
 }
@@ -640,10 +688,13 @@ int icap_distill_loss(const void* logits, int dtype, int N, int V, int rows_inne
   DistillArgs a{logits, view, teacher_logits, teacher_dtype, teacher_ids, N, V, K, temperature,
                 grad_loss, loss, dlogits, out};
   const RowShape shape = row_shape(dtype, N, V);
-#define LAUNCH(D, W, NV)                                                                       \
-  hipLaunchKernelGGL((distill_loss_kernel<D, W, NV>), row_grid(N), dim3(W * 64), 0, (hipStream_t)stream, a)
+  const bool streamed = dlogits && stream_writes(row_bytes(dtype, N, V));
+#define LAUNCH_S(D, W, NV, S)                                                                         \
+  hipLaunchKernelGGL((distill_loss_kernel<D, W, NV, S>), row_grid(N), dim3(W * 64), 0, (hipStream_t)stream, a)
+#define LAUNCH(D, W, NV) do { if (streamed) LAUNCH_S(D, W, NV, true); else LAUNCH_S(D, W, NV, false); } while (0)
   ICAP_BY_ROWS(dtype, shape, LAUNCH);
 #undef LAUNCH
+#undef LAUNCH_S
   ICAP_LAUNCH_CHECK("distill_loss_kernel");
   return ICAP_OK;
 }

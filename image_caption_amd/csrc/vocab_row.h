@@ -37,6 +37,7 @@ template <>
 struct Elem<ICAP_DTYPE_F32> {
   typedef float type;
   static constexpr int kVec = 4;
+  static constexpr uint32_t kNothing = 0xff800000u;      // 32 bits of -inf
   __device__ static float up(float v) { return v; }
   __device__ static float down(float v) { return v; }
   __device__ static void unpack(u32x4 raw, float (&x)[kVec]) {
@@ -55,6 +56,7 @@ template <>
 struct Elem<ICAP_DTYPE_BF16> {
   typedef __bf16 type;
   static constexpr int kVec = 8;
+  static constexpr uint32_t kNothing = 0xff80ff80u;
   __device__ static float up(__bf16 v) { return (float)v; }
   __device__ static __bf16 down(float v) { return (__bf16)v; }
   __device__ static void unpack(u32x4 raw, float (&x)[kVec]) {
@@ -80,6 +82,7 @@ template <>
 struct Elem<ICAP_DTYPE_F16> {
   typedef _Float16 type;
   static constexpr int kVec = 8;
+  static constexpr uint32_t kNothing = 0xfc00fc00u;
   __device__ static float up(_Float16 v) { return (float)v; }
   __device__ static _Float16 down(float v) { return (_Float16)v; }
   __device__ static void unpack(u32x4 raw, float (&x)[kVec]) {
@@ -103,6 +106,19 @@ struct Elem<ICAP_DTYPE_F16> {
   }
 };
 
+// 16 bytes from any address.  STREAM: data that nothing which follows will find in the caches - the
+// last level holds 256 MB - and that need not push out what else is there (non-temporal).  A template
+// parameter all the way: of two accesses in the branches of an if the compiler makes one.
+template <bool STREAM>
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  return STREAM ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p;
+}
+template <bool STREAM>
+__device__ __forceinline__ void store16(void* p, u32x4 v) {
+  if constexpr (STREAM) __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p);
+  else *(u32x4_any*)p = v;
+}
+
 // n elements from p on, n = kVec (one 16-byte access) or 1.  No bounds and no branch, so that a
 // batch of loads stays in flight together: the caller keeps col + n inside the row.
 template <int DTYPE, int n>
@@ -111,8 +127,9 @@ struct Piece {
   u32x4 raw;
   __device__ __forceinline__ void load(const type* p) { raw = *reinterpret_cast<const u32x4_any*>(p); }
   __device__ __forceinline__ void unpack(float (&x)[n]) const { Elem<DTYPE>::unpack(raw, x); }
+  template <bool STREAM = false>
   __device__ static __forceinline__ void store(type* p, const float (&x)[n]) {
-    *reinterpret_cast<u32x4_any*>(p) = Elem<DTYPE>::pack(x);
+    store16<STREAM>(p, Elem<DTYPE>::pack(x));
   }
 };
 template <int DTYPE>
@@ -121,6 +138,7 @@ struct Piece<DTYPE, 1> {
   type raw;
   __device__ __forceinline__ void load(const type* p) { raw = *p; }
   __device__ __forceinline__ void unpack(float (&x)[1]) const { x[0] = Elem<DTYPE>::up(raw); }
+  template <bool STREAM = false>
   __device__ static __forceinline__ void store(type* p, const float (&x)[1]) { *p = Elem<DTYPE>::down(x[0]); }
 };
 
@@ -173,17 +191,20 @@ __device__ __forceinline__ float row_ref(float m, float rate) {
   return fminf(fmaxf(m * rate, -kRefLimit), kRefLimit);
 }
 
-// A sum of products 2^y y with -inf among the y comes out as NaN; `safe` holds y at kFarBelow, which
-// costs one instruction of eight and so is left out where a look at the result tells.
-template <bool safe, int n>
+template <int n>
 __device__ __forceinline__ void row_stats_add(float& s, float& w, const float (&x)[n], float rate, float c) {
 #pragma unroll
   for (int i = 0; i < n; ++i) {
     const float y = __builtin_fmaf(x[i], rate, -c);
     const float e = __builtin_amdgcn_exp2f(y);
     s += e;
-    w = __builtin_fmaf(e, safe ? fmaxf(y, kFarBelow) : y, w);
+    w = __builtin_fmaf(e, fmaxf(y, kFarBelow), w);
   }
+}
+template <int n>
+__device__ __forceinline__ void row_sum_add(float& s, const float (&x)[n], float rate, float c) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) s += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], rate, -c));
 }
 template <int n>
 __device__ __forceinline__ float row_max(float m, const float (&x)[n]) {
@@ -268,26 +289,24 @@ __device__ __forceinline__ RowResult row_result(RowStats a, float rate, Far far)
 
 // A row in the hands of a workgroup of WAVES waves: pieces of kVec elements, thread t holding the
 // pieces t, t + threads, ..., and the V % kVec elements behind the last whole piece one each.
-// NV > 0: up to NV pieces a thread, which stay in registers, so that the row is read once
-// however often it is looked at; NV = 0: any length, read again each time.
-template <int DTYPE, int WAVES, int NV>
+// NV > 0: up to NV pieces a thread, which stay in registers, so that the row is read once;
+// NV = 0: any length, read again for the second look.
+template <int DTYPE, int WAVES, int NV, bool STREAM>
 struct Row {
   typedef Elem<DTYPE> E;
   typedef typename E::type type;
   static constexpr int kThreads = WAVES * 64;
   static constexpr int kBatch = 4;      // loads in flight of a row that is not held
-  static constexpr uint32_t kNothing = DTYPE == ICAP_DTYPE_F32    ? 0xff800000u
-                                       : DTYPE == ICAP_DTYPE_BF16 ? 0xff80ff80u
-                                                                  : 0xfc00fc00u;      // -inf
+  static constexpr bool kHeld = NV > 0;
   const type* x;
   int V, pieces;
-  u32x4 raw[NV > 0 ? NV : 1];
-  float tail;      // -inf without one
+  u32x4 raw[kHeld ? NV : 1];
+  float tail;          // -inf without one
 
   __device__ __forceinline__ u32x4 read(int i) const {
     // (a thread without an i-th piece reads the last one and forgets it: no branch round a load)
-    u32x4 r = *reinterpret_cast<const u32x4_any*>(x + (size_t)min(i, pieces - 1) * E::kVec);
-    if (i >= pieces) r = u32x4{kNothing, kNothing, kNothing, kNothing};
+    u32x4 r = load16<STREAM && kHeld>(x + (size_t)min(i, pieces - 1) * E::kVec);
+    if (i >= pieces) r = u32x4{E::kNothing, E::kNothing, E::kNothing, E::kNothing};
     return r;
   }
   __device__ __forceinline__ int tail_col() const { return pieces * E::kVec + (int)threadIdx.x; }
@@ -296,7 +315,7 @@ struct Row {
     x = row;
     V = n;
     pieces = n / E::kVec;
-    if constexpr (NV > 0) {
+    if constexpr (kHeld) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (j * kThreads < pieces) raw[j] = read(j * kThreads + threadIdx.x);
@@ -308,7 +327,7 @@ struct Row {
   // past the row's end are -inf
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    if constexpr (NV > 0) {
+    if constexpr (kHeld) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (j * kThreads < pieces) {
@@ -333,85 +352,39 @@ struct Row {
     f(v, tail_col());
   }
 
-  // This thread's part of the statistics
-  __device__ __forceinline__ RowStats stats(float rate) const {
+  // This thread's part of the sum; no entropy.
+  __device__ __forceinline__ RowStats sums(float rate) const {
     RowStats a = row_stats_empty();
-    if constexpr (NV > 0) {
+    if constexpr (kHeld) {
       each([&](const auto& v, int) { a.m = row_max(a.m, v); });
       const float c = row_ref(a.m, rate);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (j * kThreads < pieces) {
-          float v[E::kVec];
-          E::unpack(raw[j], v);
-          if ((j + 1) * kThreads <= pieces) row_stats_add<false>(a.s, a.w, v, rate, c);
-          else row_stats_add<true>(a.s, a.w, v, rate, c);
-        }
-      }
-      if (!(a.w == a.w)) {
-        a.s = a.w = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (j * kThreads < pieces) {
-            float v[E::kVec];
-            E::unpack(raw[j], v);
-            row_stats_add<true>(a.s, a.w, v, rate, c);
-          }
-        }
-      }
-      const float v[1] = {tail};
-      row_stats_add<true>(a.s, a.w, v, rate, c);
+      each([&](const auto& v, int) { row_sum_add(a.s, v, rate, c); });
     } else {
       for (int i0 = 0; i0 < pieces; i0 += kBatch * kThreads) {
-        u32x4 r[kBatch];
+        float v[kBatch][E::kVec];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) r[j] = read(i0 + j * kThreads + threadIdx.x);
+        for (int j = 0; j < kBatch; ++j) E::unpack(read(i0 + j * kThreads + threadIdx.x), v[j]);
         float m = a.m;
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          float v[E::kVec];
-          E::unpack(r[j], v);
-          m = row_max(m, v);
-        }
+        for (int j = 0; j < kBatch; ++j) m = row_max(m, v[j]);
         const float c = row_ref(m, rate);
         row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
         a.m = m;
-        const float s = a.s, w = a.w;
-        // (unpacked again below: held unpacked they would cost 32 registers and half the waves)
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) asm volatile("" : "+v"(r[j]));
-        const bool whole = i0 + kBatch * kThreads <= pieces;
-        if (whole) {
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            float v[E::kVec];
-            E::unpack(r[j], v);
-            row_stats_add<false>(a.s, a.w, v, rate, c);
-          }
-        }
-        if (!whole || !(a.w == a.w)) {
-          a.s = s;
-          a.w = w;
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            float v[E::kVec];
-            E::unpack(r[j], v);
-            row_stats_add<true>(a.s, a.w, v, rate, c);
-          }
-        }
+        for (int j = 0; j < kBatch; ++j) row_sum_add(a.s, v[j], rate, c);
       }
       const float v[1] = {tail};
       const float m = row_max(a.m, v), c = row_ref(m, rate);
       row_stats_move(a.s, a.w, row_ref(a.m, rate), c);
       a.m = m;
-      row_stats_add<true>(a.s, a.w, v, rate, c);
+      row_sum_add(a.s, v, rate, c);
     }
     return a;
   }
 
-  // The row's statistics, the same in every thread
+  // The row's statistics, the same in every thread (entropy: not among them)
   __device__ __forceinline__ RowResult result(float rate, RowStats* s_part) const {
-    return row_result(row_stats_block<WAVES>(stats(rate), rate, s_part), rate, [&](float m) {
+    return row_result(row_stats_block<WAVES>(sums(rate), rate, s_part), rate, [&](float m) {
       RowStats f = {m, 0.f, 0.f};
       for (int i = threadIdx.x; i < V; i += kThreads) row_stats_add_far(f, E::up(x[i]), rate);
       if constexpr (WAVES > 1) __syncthreads();
@@ -419,27 +392,34 @@ struct Row {
     });
   }
 
-  // out[column] = f(value, column) in the row's type; out may be the row itself once it was opened
-  // (each thread writes what it alone read)
-  template <class F>
-  __device__ __forceinline__ void write(type* out, F f) const {
+  // out[column] = factor * exp((value - m) / tau - log_s) in the row's type; out may be the row
+  // itself (each thread writes what it alone read)
+  __device__ __forceinline__ void write_softmax(type* out, const RowResult& r, float rate, float factor) const {
+    const float m = r.m, inv_s = factor * __builtin_amdgcn_exp2f(-r.log_s * kLog2e);
     each([&](const auto& v, int c) {
       constexpr int n = sizeof(v) / sizeof(float);
       if (c + n > V) return;
       float g[n];
 #pragma unroll
-      for (int e = 0; e < n; ++e) g[e] = f(v[e], c + e);
-      Piece<DTYPE, n>::store(out + c, g);
+      for (int e = 0; e < n; ++e) g[e] = __builtin_amdgcn_exp2f((v[e] - m) * rate) * inv_s;
+      Piece<DTYPE, n>::template store<STREAM>(out + c, g);
     });
   }
 };
 
+// Whether a call's reads or writes count as a stream.  Measured with the next operator reading the
+// result: written past the caches a lookup's 134 MB take 28 instead of 38 us and both together 82
+// instead of 84, 67 MB 41.4 against 41.4; read past them 410 MB of logits take 64 instead of 73 us,
+// but at 195 MB a gradient that follows loses more than that gains.
+inline bool stream_reads(size_t bytes) { return bytes > (size_t)256 << 20; }
+inline bool stream_writes(size_t bytes) { return bytes > (size_t)96 << 20; }
+
 // Zeros in a row of V elements.
-template <int DTYPE, int WAVES>
+template <int DTYPE, int WAVES, bool STREAM>
 __device__ __forceinline__ void write_zeros(typename Elem<DTYPE>::type* out, int V) {
   constexpr int n = Elem<DTYPE>::kVec;
   const float zero[n] = {}, one[1] = {};
-  for (int i = threadIdx.x; i < V / n; i += WAVES * 64) Piece<DTYPE, n>::store(out + (size_t)i * n, zero);
+  for (int i = threadIdx.x; i < V / n; i += WAVES * 64) Piece<DTYPE, n>::template store<STREAM>(out + (size_t)i * n, zero);
   const int c = V / n * n + (int)threadIdx.x;
   if (c < V) Piece<DTYPE, 1>::store(out + c, one);
 }
