@@ -70,72 +70,188 @@ struct SortArgs {
   int32_t* row_start;
   int2* sorted;               // (position, token)
   int32_t* long_count;
+  int2* split;                // embed_split_kernel's lists and where each workgroup's tokens begin in them
+  int32_t* split_start;
+  int split_lists;
 };
 
-// Workgroup b reads all N tokens - 16 waves, a share of the positions each - and counts how many
+__device__ __forceinline__ bool takes_part(int id, int V, int pad) {
+  return (unsigned)id < (unsigned)V && id != pad;
+}
+
+// The lanes whose key has the same low bits, among those that take part.
+__device__ __forceinline__ unsigned long long same_key(int key, int bits, bool part) {
+  unsigned long long same = __ballot(part);
+  for (int i = 0; i < bits; ++i) {
+    const unsigned long long one = __ballot((key >> i) & 1);
+    same &= (key >> i) & 1 ? one : ~one;
+  }
+  return same;
+}
+
+constexpr int kSplitTokens = 2048;      // of a list
+constexpr int kSplitLists = 1024;
+
+// Lists of kSplitTokens tokens in a row, each ordered by the workgroup of embed_sort_kernel that
+// will take a token, positions ascending: that kernel then reads its own tokens only.
+__global__ __launch_bounds__(kSortWaves * 64) void embed_split_kernel(SortArgs p) {
+  __shared__ int s_cnt[kSortWaves][256];
+  __shared__ int s_wave[4];
+  constexpr int kSteps = kSplitTokens / (kSortWaves * 64);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const unsigned long long lower = (1ull << lane) - 1;
+  for (int i = tid; i < kSortWaves * 256; i += kSortWaves * 64) (&s_cnt[0][0])[i] = 0;
+  __syncthreads();
+  const int from = blockIdx.x * kSplitTokens + wave * 64 * kSteps + lane;
+  int id[kSteps], at[kSteps];
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    id[j] = p.ids[min(from + j * 64, p.N - 1)];
+    if (from + j * 64 >= p.N || !takes_part(id[j], p.V, p.pad)) id[j] = -1;
+  }
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    const unsigned long long same = same_key(id[j], 8, id[j] >= 0);
+    const int leader = __ffsll(same) - 1;
+    int begin = 0;
+    if (id[j] >= 0 && lane == leader) begin = atomicAdd(&s_cnt[wave][id[j] & 255], __popcll(same));
+    at[j] = __shfl(begin, max(leader, 0), 64) + __popcll(same & lower);
+  }
+  __syncthreads();
+  int total = 0, upto = 0;
+  if (tid < 256) {
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = s_cnt[w][tid];
+      s_cnt[w][tid] = total;
+      total += c;
+    }
+    upto = total;      // inclusive scan over the 256 keys
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 63) s_wave[wave] = upto;
+  }
+  __syncthreads();
+  if (tid < 256) {
+    for (int w = 0; w < wave; ++w) upto += s_wave[w];
+    const int begin = upto - total;
+    for (int w = 0; w < kSortWaves; ++w) s_cnt[w][tid] += begin;
+    p.split_start[blockIdx.x * 257 + tid] = begin;
+    if (tid == 255) p.split_start[blockIdx.x * 257 + 256] = upto;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j)
+    if (id[j] >= 0)
+      p.split[(size_t)blockIdx.x * kSplitTokens + s_cnt[wave][id[j] & 255] + at[j]] = make_int2(from + j * 64, id[j]);
+}
+
+// Workgroup b goes through the tokens - 16 waves, a share of the positions each - and counts how many
 // belong to earlier workgroups and, per wave and row, how many to this one; its own tokens it
 // notes in LDS, in order.  Then it writes them behind those counts, in ascending order of their
 // positions within a row.  A wave whose own tokens overflow its list (one word filling the
 // batch) reads its share again instead.  Every count is an integer and every place follows from
 // the counts, so nothing depends on timing, and no workgroup waits for another.
-// (256 x N tokens are read in all, from the caches: at N = 131072 one workgroup's 512 kB take
-// about as long as the compare instructions on them.)
+// SPLIT: its tokens come from the lists of embed_split_kernel.  Otherwise it reads all of them, 256 x N
+// in all from the caches, which for few tokens is less than a launch: 10240 take 8 us, 131071 took
+// 34 us and take 12 by way of the lists.
+template <bool SPLIT>
 __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(SortArgs p) {
   __shared__ int s_cnt[kSortWaves][kSortRows];
   __shared__ int2 s_list[kSortWaves][kSortList];
   __shared__ int s_wave[kSortWaves];
+  __shared__ int s_upto[SPLIT ? kSortWaves : 1][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x, mask = (1 << p.slots.bits) - 1, rows = p.slots.rows;
   for (int i = tid; i < kSortWaves * rows; i += kSortWaves * 64) s_cnt[i / rows][i % rows] = 0;
   if (b == 0 && tid == 0) *p.long_count = 0;
   __syncthreads();
+  const unsigned long long lower = (1ull << lane) - 1;
+  int below = 0, noted = 0;
+  // all tokens: this wave's positions are [from, to)
   const int per = ((p.N + kSortWaves - 1) / kSortWaves + 255) / 256 * 256;
   const int from = min(p.N, wave * per), to = min(p.N, from + per);
-  const unsigned long long lower = (1ull << lane) - 1;
-  // tokens i0 + lane * 4 + 0 .. 3; one that takes no part becomes -1, which belongs to no workgroup
-  auto read = [&](int i0, int (&id)[4]) {
-    const int i = i0 + lane * 4;
-    if (i0 + 256 <= to) {
-      typedef int int4_any __attribute__((ext_vector_type(4), aligned(4)));
-      const int4_any x = *reinterpret_cast<const int4_any*>(p.ids + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) id[e] = x[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) id[e] = i + e < to ? p.ids[min(i + e, p.N - 1)] : -1;
-    }
+  // lists: this wave's are [first, first + mine), lane i knows the i-th one's part for b
+  const int lists = (p.split_lists + kSortWaves - 1) / kSortWaves;
+  const int first = wave * lists;
+  int part_begin = 0;
+  auto from_lists = [&](int t) {      // the wave's t-th token
+    int l = 0;                        // the first list that reaches past t
+    for (int step = 32; step > 0; step >>= 1)
+      if (s_upto[wave][l + step - 1] <= t) l += step;
+    const int before = l ? s_upto[wave][l - 1] : 0;
+    const int begin = __shfl(part_begin, l, 64);
+    return p.split[(size_t)(first + l) * kSplitTokens + begin + t - before];
   };
-  auto valid = [&](int id) { return (unsigned)id < (unsigned)p.V && id != p.pad; };
-  int below = 0, noted = 0;
-  auto count = [&](int i0, const int (&id)[4]) {
-    unsigned long long m[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool ok = valid(id[e]);
-      below += ok && (id[e] & mask) < b;
-      m[e] = __ballot(ok && (id[e] & mask) == b);
+  if constexpr (SPLIT) {
+    const bool there = lane < lists && first + lane < p.split_lists;
+    int size = 0;
+    if (there) {
+      const int32_t* at = p.split_start + (size_t)(first + lane) * 257 + b;
+      part_begin = at[0];
+      size = at[1] - part_begin;
+      below = part_begin;
     }
-    if (!(m[0] | m[1] | m[2] | m[3])) return;
-    int at = noted;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      at += __popcll(m[e] & lower);
-      noted += __popcll(m[e]);
+    int upto = size;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((m[e] >> lane) & 1) {
-        atomicAdd(&s_cnt[wave][id[e] >> p.slots.bits], 1);
-        if (at < kSortList) s_list[wave][at] = make_int2(i0 + lane * 4 + e, id[e]);
-        ++at;
+    s_upto[wave][lane] = upto;
+    noted = __shfl(upto, 63, 64);
+    __syncthreads();
+    for (int t0 = 0; t0 < noted; t0 += 64) {
+      const int2 x = from_lists(min(t0 + lane, noted - 1));
+      if (t0 + lane < noted) {
+        atomicAdd(&s_cnt[wave][x.y >> p.slots.bits], 1);
+        if (t0 + lane < kSortList) s_list[wave][t0 + lane] = x;
       }
-  };
-  for (int i0 = from; i0 < to; i0 += 256 * kSortAhead) {
-    int id[kSortAhead][4];
+    }
+  } else {
+    // tokens i0 + lane * 4 + 0 .. 3
+    auto read = [&](int i0, int (&id)[4]) {
+      const int i = i0 + lane * 4;
+      if (i0 + 256 <= to) {
+        typedef int int4_any __attribute__((ext_vector_type(4), aligned(4)));
+        const int4_any x = *reinterpret_cast<const int4_any*>(p.ids + i);
 #pragma unroll
-    for (int j = 0; j < kSortAhead; ++j) read(i0 + j * 256, id[j]);
+        for (int e = 0; e < 4; ++e) id[e] = x[e];
+      } else {
 #pragma unroll
-    for (int j = 0; j < kSortAhead; ++j) count(i0 + j * 256, id[j]);
+        for (int e = 0; e < 4; ++e) id[e] = i + e < to ? p.ids[min(i + e, p.N - 1)] : -1;
+      }
+    };
+    auto count = [&](int i0, const int (&id)[4]) {
+      unsigned long long m[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool ok = takes_part(id[e], p.V, p.pad);
+        below += ok && (id[e] & mask) < b;
+        m[e] = __ballot(ok && (id[e] & mask) == b);
+      }
+      if (!(m[0] | m[1] | m[2] | m[3])) return;
+      int at = noted;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        at += __popcll(m[e] & lower);
+        noted += __popcll(m[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((m[e] >> lane) & 1) {
+          atomicAdd(&s_cnt[wave][id[e] >> p.slots.bits], 1);
+          if (at < kSortList) s_list[wave][at] = make_int2(i0 + lane * 4 + e, id[e]);
+          ++at;
+        }
+    };
+    for (int i0 = from; i0 < to; i0 += 256 * kSortAhead) {
+      int id[kSortAhead][4];
+#pragma unroll
+      for (int j = 0; j < kSortAhead; ++j) read(i0 + j * 256, id[j]);
+#pragma unroll
+      for (int j = 0; j < kSortAhead; ++j) count(i0 + j * 256, id[j]);
+    }
   }
   for (int d = 32; d > 0; d >>= 1) below += __shfl_xor(below, d, 64);
   if (lane == 0) s_wave[wave] = below;
@@ -165,29 +281,25 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(SortArgs p)
     }
   }
   __syncthreads();
-  // 64 tokens of one wave, in the order of the lanes; id -1: none
-  auto place = [&](int i, int id) {
-    unsigned long long left = __ballot(id >= 0);
-    while (left) {        // the lanes of one id at a time
-      const int leader = __ffsll(left) - 1;
-      const int r = __builtin_amdgcn_readlane(id, leader);
-      const unsigned long long same = __ballot(id == r);
-      int at = 0;
-      if (lane == leader) at = atomicAdd(&s_cnt[wave][r >> p.slots.bits], __popcll(same));
-      at = __builtin_amdgcn_readlane(at, leader);
-      if (id == r) p.sorted[at + __popcll(same & lower)] = make_int2(i, id);
-      left &= ~same;
-    }
+  // 64 tokens of one wave, in the order of the lanes
+  const int row_bits = 32 - __builtin_clz(rows);
+  auto place = [&](int2 t, bool part) {
+    const int r = t.y >> p.slots.bits;
+    const unsigned long long same = same_key(r, row_bits, part);
+    const int leader = __ffsll(same) - 1;
+    int at = 0;
+    if (part && lane == leader) at = atomicAdd(&s_cnt[wave][r], __popcll(same));
+    at = __shfl(at, max(leader, 0), 64);
+    if (part) p.sorted[at + __popcll(same & lower)] = t;
   };
   if (noted <= kSortList) {
-    for (int k = 0; k < noted; k += 64) {
-      const int2 t = s_list[wave][min(k + lane, noted - 1)];
-      place(t.x, k + lane < noted ? t.y : -1);
-    }
+    for (int k = 0; k < noted; k += 64) place(s_list[wave][min(k + lane, noted - 1)], k + lane < noted);
+  } else if constexpr (SPLIT) {
+    for (int k = 0; k < noted; k += 64) place(from_lists(min(k + lane, noted - 1)), k + lane < noted);
   } else {
     for (int i = from; i < to; i += 64) {
       const int id = p.ids[min(i + lane, to - 1)];
-      place(i + lane, i + lane < to && valid(id) && (id & mask) == b ? id : -1);
+      place(make_int2(i + lane, id), i + lane < to && takes_part(id, p.V, p.pad) && (id & mask) == b);
     }
   }
 }
@@ -200,7 +312,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(SortArgs p)
 // `part` for each chunk it reaches (slot 0: the row of the chunk's first token, slot 1: the row of
 // its last one, if another); the chunk where it starts puts it on the list of long rows, and
 // embed_join_kernel adds its shares up in the chunks' order.  Rows without tokens get their zeros
-// from further groups, 64 slots each.
+// from further waves, kZeroSlots of them each.
 struct SumArgs {
   const void* grad;
   void* dtable;
@@ -215,6 +327,7 @@ struct SumArgs {
 };
 
 constexpr int kSumAhead = 8;
+constexpr int kZeroSlots = 16;       // rows that a wave looks over for ones without tokens
 
 template <int DTYPE, int n>
 __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs p) {
@@ -224,11 +337,12 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs p) {
   const int sums = p.chunks * p.col_blocks, sum_blocks = (sums + groups - 1) / groups;
   typename P::type* table = (typename P::type*)p.dtable;
   if ((int)blockIdx.x >= sum_blocks) {
-    const int slot0 = ((int)blockIdx.x - sum_blocks) * 256 + (threadIdx.x & ~63), slot = slot0 + (threadIdx.x & 63);
+    const int slot0 = (((int)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * kZeroSlots;
+    const int slot = slot0 + (threadIdx.x & 63);
     const bool empty = slot < p.slots.count() && p.row_start[slot] == p.row_start[slot + 1];
     const unsigned long long mask = __ballot(empty);
     const float zero[n] = {};
-    for (int r = (threadIdx.x & 63) / p.lanes; r < 64; r += 64 / p.lanes) {
+    for (int r = (threadIdx.x & 63) / p.lanes; r < kZeroSlots; r += 64 / p.lanes) {
       const int v = p.slots.row(slot0 + r);
       if (!((mask >> r) & 1) || v >= p.V) continue;
       for (int c = lane * n; c < p.D; c += p.lanes * n)
@@ -347,8 +461,14 @@ Slots slots_of(int V) {
 }
 
 struct Workspace {
-  size_t row_start, sorted, long_rows, part, bytes;
+  size_t row_start, sorted, long_rows, part, split, split_start, bytes;
 };
+
+// Whether the tokens go through lists: from where reading all of them 256 times costs more than a
+// launch, as long as the lists' part for a workgroup fits the lanes that look it up.
+bool splits(int N, int V) {
+  return N > 24576 && ceil_div(N, kSplitTokens) <= kSplitLists && slots_of(V).bits == 8;
+}
 
 Workspace workspace_of(int N, int V, int D) {
   const size_t chunks = (size_t)ceil_div(N, chunk_of(N));
@@ -358,7 +478,9 @@ Workspace workspace_of(int N, int V, int D) {
   w.sorted = w.row_start + pad16(((size_t)slots_of(V).count() + 1) * sizeof(int32_t));
   w.long_rows = w.sorted + pad16((size_t)N * sizeof(int2));
   w.part = w.long_rows + pad16((chunks + 1) * sizeof(int32_t));      // their number, then the rows
-  w.bytes = w.part + chunks * 2 * (size_t)D * sizeof(float);
+  w.split = w.part + pad16(chunks * 2 * (size_t)D * sizeof(float));
+  w.split_start = w.split + (splits(N, V) ? (size_t)ceil_div(N, kSplitTokens) * kSplitTokens * sizeof(int2) : 0);
+  w.bytes = w.split_start + (splits(N, V) ? (size_t)ceil_div(N, kSplitTokens) * 257 * sizeof(int32_t) : 0);
   return w;
 }
 
@@ -440,8 +562,17 @@ int icap_embedding_grad(const void* grad, int dtype, const int32_t* ids, void* d
   int32_t* long_count = (int32_t*)(ws + w.long_rows);
   hipStream_t s = (hipStream_t)stream;
   const Slots slots = slots_of(V);
-  hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << slots.bits), dim3(kSortWaves * 64), 0, s,
-                     SortArgs{ids, N, V, pad_token, slots, row_start, sorted, long_count});
+  const bool split = splits(N, V);
+  SortArgs sort{ids, N, V, pad_token, slots, row_start, sorted, long_count, (int2*)(ws + w.split),
+                (int32_t*)(ws + w.split_start), split ? ceil_div(N, kSplitTokens) : 0};
+  const dim3 sort_grid(1u << slots.bits), sort_block(kSortWaves * 64);
+  if (split) {
+    hipLaunchKernelGGL(embed_split_kernel, dim3(sort.split_lists), sort_block, 0, s, sort);
+    ICAP_LAUNCH_CHECK("embed_split_kernel");
+    hipLaunchKernelGGL(embed_sort_kernel<true>, sort_grid, sort_block, 0, s, sort);
+  } else {
+    hipLaunchKernelGGL(embed_sort_kernel<false>, sort_grid, sort_block, 0, s, sort);
+  }
   ICAP_LAUNCH_CHECK("embed_sort_kernel");
   const int vec = vec_of(dtype, D), lanes = lanes_of(D, vec);
   const int chunk = chunk_of(N), chunks = ceil_div(N, chunk);
@@ -449,7 +580,7 @@ int icap_embedding_grad(const void* grad, int dtype, const int32_t* ids, void* d
             slots, V, D, chunk, chunks, lanes, ceil_div(D, lanes * vec), scale};
   const int groups = 256 / lanes;
   const dim3 grid((unsigned)(((long long)chunks * a.col_blocks + groups - 1) / groups +
-                             ceil_div(slots.count(), 256)));
+                             ceil_div(slots.count(), 4 * kZeroSlots)));
   const dim3 join((unsigned)std::max(1LL, std::min(1024LL, (long long)chunks * ceil_div(D, 64))));
 #define LAUNCH(T, n)                                                                   \
   do {                                                                                 \

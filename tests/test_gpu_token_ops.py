@@ -458,6 +458,17 @@ def test_embedding_gradient_of_tokens_that_fill_the_batch(kind, N, V, D):
     assert not none.any()
 
 
+@pytest.mark.parametrize("N,V,D", [(24576, 300, 8), (24577, 300, 8), (26624, 131072, 4), (26625, 131073, 4), (50000, 1, 3),
+                                   (100003, 5000, 12), (300000, 50000, 4)])
+def test_embedding_gradient_of_long_batches(N, V, D):
+    """Around the length from which the tokens are sorted by way of lists, and the largest table for that."""
+    rng = np.random.default_rng(N)
+    grad = _logits(rng, N, D, "f32", 1.0)
+    _check_embed_grad(grad, rng.integers(-1, V + 1, N), V, 2.0, -1, "f32", "uniform")
+    _check_embed_grad(grad, np.minimum(rng.zipf(1.2, N) - 1, V - 1), V, 1.0, 0, "f32", "by frequency")
+    _check_embed_grad(grad, np.full(N, V // 2), V, 1.0, -1, "f32", "one token")
+
+
 def test_embedding_gradient_of_padding_that_holds_nan_and_of_nothing():
     from image_caption_amd import ops
     grad = torch.ones(4, 8, device=dev())
