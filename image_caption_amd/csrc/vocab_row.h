@@ -125,7 +125,8 @@ template <int DTYPE, int n>
 struct Piece {
   typedef typename Elem<DTYPE>::type type;
   u32x4 raw;
-  __device__ __forceinline__ void load(const type* p) { raw = *reinterpret_cast<const u32x4_any*>(p); }
+  template <bool STREAM = false>
+  __device__ __forceinline__ void load(const type* p) { raw = load16<STREAM>(p); }
   __device__ __forceinline__ void unpack(float (&x)[n]) const { Elem<DTYPE>::unpack(raw, x); }
   template <bool STREAM = false>
   __device__ static __forceinline__ void store(type* p, const float (&x)[n]) {
@@ -136,6 +137,7 @@ template <int DTYPE>
 struct Piece<DTYPE, 1> {
   typedef typename Elem<DTYPE>::type type;
   type raw;
+  template <bool STREAM = false>
   __device__ __forceinline__ void load(const type* p) { raw = *p; }
   __device__ __forceinline__ void unpack(float (&x)[1]) const { x[0] = Elem<DTYPE>::up(raw); }
   template <bool STREAM = false>

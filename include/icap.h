@@ -572,7 +572,7 @@ int icap_sample_categorical_f32(const float* logits, const float* u, const int32
 
 /* ---- what a decoder is trained with ---------------------------------------------------
  * The reference trains its decoders in TensorFlow (teacher forcing recurrent_example.py:381-475,
- * REINFORCE / self-critical / actor-critic utils/train_utils.py:397-515 on the samples of
+ * REINFORCE / self-critical / actor-critic utils/train_utils.py:397,432,476 on the samples of
  * utils/agent_utils.py); these are the operators at the two ends of such a step, forward and
  * gradient, plus distillation.  `dtype` is the ICAP_DTYPE_* of the logits (table), statistics
  * and losses are float32.  Logits are rows of V elements: row r starts at element
