@@ -411,9 +411,9 @@ __device__ __forceinline__ void gemm_bf16_body(const Bf16Args& p, const int bid,
         if (p.gru) {
           const float zg = fast_sigmoid(z[0]), rg = fast_sigmoid(z[1]);
           const float hh = fast_tanh(z[2] + rg * z[3]);
-          p.h_out[o] = zg * st_pre[q] + (1.f - zg) * hh;
+          p.h_out[o] = sum_of_products(zg, st_pre[q], 1.f - zg, hh);
         } else {
-          const float cn = fast_sigmoid(z[1]) * st_pre[q] + fast_sigmoid(z[0]) * fast_tanh(z[2]);
+          const float cn = sum_of_products(fast_sigmoid(z[1]), st_pre[q], fast_sigmoid(z[0]), fast_tanh(z[2]));
           p.c_out[o] = cn;
           p.h_out[o] = fast_sigmoid(z[3]) * fast_tanh(cn);
         }
@@ -831,9 +831,9 @@ __global__ __launch_bounds__(256) void cell_update_kernel(const float* __restric
   if (gru) {
     const float zg = fast_sigmoid(zz[0]), rg = fast_sigmoid(zz[1]);
     const float hh = fast_tanh(zz[2] + rg * zz[3]);
-    h_out[idx] = zg * st + (1.f - zg) * hh;
+    h_out[idx] = sum_of_products(zg, st, 1.f - zg, hh);
   } else {
-    const float cn = fast_sigmoid(zz[1]) * st + fast_sigmoid(zz[0]) * fast_tanh(zz[2]);
+    const float cn = sum_of_products(fast_sigmoid(zz[1]), st, fast_sigmoid(zz[0]), fast_tanh(zz[2]));
     c_out[idx] = cn;
     h_out[idx] = fast_sigmoid(zz[3]) * fast_tanh(cn);
   }

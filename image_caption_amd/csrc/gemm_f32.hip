@@ -962,14 +962,14 @@ __device__ __forceinline__ void cell_update(const LstmArgs& p, size_t o, float z
     const float fg = fast_sigmoid(z1);
     const float gg = fast_tanh(z2);
     const float og = fast_sigmoid(z3);
-    const float c_new = fg * p.c[o] + ig * gg;
+    const float c_new = sum_of_products(fg, p.c[o], ig, gg);
     p.c_out[o] = c_new;
     p.h_out[o] = og * fast_tanh(c_new);
   } else {
     const float zg = fast_sigmoid(z0);
     const float rg = fast_sigmoid(z1);
     const float hh = fast_tanh(z2 + rg * z3);
-    p.h_out[o] = zg * p.h[o] + (1.f - zg) * hh;
+    p.h_out[o] = sum_of_products(zg, p.h[o], 1.f - zg, hh);
   }
 }
 
@@ -982,14 +982,14 @@ __device__ __forceinline__ void cell_update_pre(const LstmArgs& p, size_t o, flo
     const float fg = fast_sigmoid(z1);
     const float gg = fast_tanh(z2);
     const float og = fast_sigmoid(z3);
-    const float c_new = fg * prev + ig * gg;
+    const float c_new = sum_of_products(fg, prev, ig, gg);
     p.c_out[o] = c_new;
     p.h_out[o] = og * fast_tanh(c_new);
   } else {
     const float zg = fast_sigmoid(z0);
     const float rg = fast_sigmoid(z1);
     const float hh = fast_tanh(z2 + rg * z3);
-    p.h_out[o] = zg * prev + (1.f - zg) * hh;
+    p.h_out[o] = sum_of_products(zg, prev, 1.f - zg, hh);
   }
 }
 

@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256, 2) void gemm_split_kernel(SplitArgs p) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) z[g] += bz[g];
       const size_t o = (size_t)m * H + unit;
-      const float cn = fast_sigmoid(z[1]) * p.c_in[o] + fast_sigmoid(z[0]) * fast_tanh(z[2]);
+      const float cn = sum_of_products(fast_sigmoid(z[1]), p.c_in[o], fast_sigmoid(z[0]), fast_tanh(z[2]));
       p.c_out[o] = cn;
       p.h_out[o] = fast_sigmoid(z[3]) * fast_tanh(cn);
     }

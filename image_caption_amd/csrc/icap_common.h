@@ -59,6 +59,14 @@ __device__ __forceinline__ float fast_tanh(float x) {
   return 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
 }
 
+// a*b + c*d with both products rounded.  The cell updates are built into several kernels that must
+// agree bit for bit; left to itself the compiler fuses one of the products or neither, as the code
+// around it falls.
+__device__ __forceinline__ float sum_of_products(float a, float b, float c, float d) {
+#pragma clang fp contract(off)
+  return a * b + c * d;
+}
+
 // Wave64 reductions on DPP (no LDS traffic, ~6 short VALU steps): an inclusive scan by
 // row_shr 1,2,4,8 inside each row of 16 lanes, then row_bcast15 / row_bcast31 carry the
 // row totals upward, so lane 63 ends with the reduction of all 64 lanes; v_readlane

@@ -180,7 +180,8 @@ __device__ __forceinline__ void cell_block(const SmallLoopArgs& p, int blk, int 
         z[g] = (Z2[row][g * 8 + u] + (tok ? e : 0.f)) + p.cell_bias[g * p.H + j];
       }
       const size_t o = (size_t)m * p.H + j;
-      const float c_new = fast_sigmoid(z[1]) * ld_dev(p.c + o) + fast_sigmoid(z[0]) * fast_tanh(z[2]);
+      const float c_new =
+          sum_of_products(fast_sigmoid(z[1]), ld_dev(p.c + o), fast_sigmoid(z[0]), fast_tanh(z[2]));
       st_dev(p.c + o, c_new);
       st_dev(h_out + o, fast_sigmoid(z[3]) * fast_tanh(c_new));
     }

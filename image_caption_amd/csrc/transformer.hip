@@ -116,9 +116,12 @@ __device__ __forceinline__ void store_chunk(float* p, const float (&e)[CH], floa
     reinterpret_cast<float4*>(p)[q] = make_float4(e[4 * q] * scale, e[4 * q + 1] * scale,
                                                   e[4 * q + 2] * scale, e[4 * q + 3] * scale);
 }
-// Dot product of two chunks, summed over the lph adjacent lanes that share a head.
+// Dot product of two chunks, summed over the lph adjacent lanes that share a head.  Every product is
+// rounded by itself, and what is fused in Online::add is written so: the results do not hang on what
+// the compiler makes of the code around.
 template <int CH>
 __device__ __forceinline__ float head_dot(const float (&a)[CH], const Chunk<CH>& b, int lph) {
+#pragma clang fp contract(off)
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) s += a[i] * b.e[i];
@@ -140,9 +143,9 @@ struct Online {
     const float mn = fmaxf(m, s);
     const float c = (m > -INFINITY) ? fast_exp(m - mn) : 0.f;
     const float w = fast_exp(s - mn);
-    l = l * c + w;
+    l = __builtin_fmaf(l, c, w);
 #pragma unroll
-    for (int i = 0; i < CH; ++i) acc[i] = acc[i] * c + w * v.e[i];
+    for (int i = 0; i < CH; ++i) acc[i] = __builtin_fmaf(w, v.e[i], acc[i] * c);
     m = mn;
   }
 };
