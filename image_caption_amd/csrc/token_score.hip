@@ -550,13 +550,14 @@ int waves_per_row(int dtype, int N, int V) {
   return P;
 }
 
-// Waves for a row and pieces a thread holds: as few waves as keep some 10 pieces a thread or less, 16 of
-// them with 7 while two such workgroups fit a compute unit, and longer rows read twice.  Few rows
-// go to large workgroups: their time is that of one row.  Measured, us, with the floor of one read and
-// one write in brackets: 40000 rows of 2000 in fp32 148 (121) by 2 waves of 4, 156 by 1 of 8, 162 by 4
-// of 4; 10240 of 10000 in fp32 165 (155) by 8 of 5, 175 by 4 of 10; in bf16 96 (77) by 4 of 10, 118 by 8
-// of 5; 2560 of 50000 in bf16 121 (97) by 16 of 7 or 8 of 13, 165 by 16 of 13; 2048 of 50000 in fp32
-// 201 (155) read twice, 201 by 16 of 13.
+// Waves for a row and pieces a thread holds: as few waves as keep some 10 pieces a thread or less, more
+// where two or three such rows still fit a compute unit's registers, and longer rows read twice.
+// Few rows go to large workgroups: their time is that of one row.  Measured, us, with one read and one
+// write of the logits at the rate of a copy in brackets: 40000 rows of 2000 in fp32 140 (121) by 2
+// waves of 4, 156 by 1 of 8, 162 by 4 of 4; 10240 of 10000 in fp32 162 (155) by 8 of 5, 166 by 4 of 10; in
+// bf16 94 (77) by 4 of 10, 117 by 8 of 5; 2560 of 50000 in bf16 108 (97) by 8 of 13, 115 by 16 of 7, 113 by
+// 4 of 25; 4000 of 20000 in fp32 121 (121) by 16 of 7, 128 by 8 of 13; 2048 of 50000 in fp32 189 (155)
+// read twice, 201 by 16 of 13.
 struct RowShape {
   int waves, held;
 };
@@ -567,6 +568,7 @@ RowShape row_shape(int dtype, int N, int V) {
   if (many && pieces <= 128 * 4) return {2, 4};
   if (pieces <= 256 * (many ? 4 : 2)) return {4, 4};
   if (many && pieces <= 512 * 5) return dtype == ICAP_DTYPE_F32 ? RowShape{8, 5} : RowShape{4, 10};
+  if (many && pieces <= 512 * 13 && dtype != ICAP_DTYPE_F32) return {8, 13};
   if (pieces <= 1024 * 7) return {16, 7};
   return {16, 0};
 }
@@ -576,7 +578,7 @@ RowShape row_shape(int dtype, int N, int V) {
     if ((shape).waves == 1) call(D, 1, 4);         \
     else if ((shape).waves == 2) call(D, 2, 4);    \
     else if ((shape).waves == 4) { if ((shape).held == 4) call(D, 4, 4); else call(D, 4, 10); } \
-    else if ((shape).waves == 8) call(D, 8, 5);    \
+    else if ((shape).waves == 8) { if ((shape).held == 5) call(D, 8, 5); else call(D, 8, 13); } \
     else if ((shape).held == 7) call(D, 16, 7);    \
     else call(D, 16, 0);                           \
   } while (0)

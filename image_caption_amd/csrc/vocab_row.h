@@ -271,16 +271,21 @@ struct RowResult {
   float log_s;      // ln sum exp((x - m) / tau)
   float entropy;
   bool none;        // every element is -inf
+  bool far;         // c stands too far out for rate * x - c to tell the elements apart
+  float c, s;       // unless far: the reference, and the sum relative to it
 };
 template <class Far>
 __device__ __forceinline__ RowResult row_result(RowStats a, float rate, Far far) {
   const float c = row_ref(a.m, rate);
   float off = __builtin_fmaf(a.m, rate, -c);      // of the maximum from the reference
-  if (!(fabsf(c) < kRefLimit)) {
+  RowResult r;
+  r.far = !(fabsf(c) < kRefLimit);
+  if (r.far) {
     a = far(a.m);
     off = 0.f;
   }
-  RowResult r;
+  r.c = c;
+  r.s = a.s;
   const float log_s = logf(a.s);
   r.none = a.s == 0.f;
   r.m = r.none ? -INFINITY : a.m;
@@ -397,14 +402,20 @@ struct Row {
   // out[column] = factor * exp((value - m) / tau - log_s) in the row's type; out may be the row
   // itself (each thread writes what it alone read)
   __device__ __forceinline__ void write_softmax(type* out, const RowResult& r, float rate, float factor) const {
-    const float m = r.m, inv_s = factor * __builtin_amdgcn_exp2f(-r.log_s * kLog2e);
-    each([&](const auto& v, int c) {
+    if (r.far) {
+      const float inv_s = factor * __builtin_amdgcn_exp2f(-r.log_s * kLog2e);
+      for (int i = threadIdx.x; i < V; i += kThreads)
+        out[i] = E::down(__builtin_amdgcn_exp2f((E::up(x[i]) - r.m) * rate) * inv_s);
+      return;
+    }
+    const float c = r.c, inv_s = factor / r.s;
+    each([&](const auto& v, int col) {
       constexpr int n = sizeof(v) / sizeof(float);
-      if (c + n > V) return;
+      if (col + n > V) return;
       float g[n];
 #pragma unroll
-      for (int e = 0; e < n; ++e) g[e] = __builtin_amdgcn_exp2f((v[e] - m) * rate) * inv_s;
-      Piece<DTYPE, n>::template store<STREAM>(out + c, g);
+      for (int e = 0; e < n; ++e) g[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], rate, -c)) * inv_s;
+      Piece<DTYPE, n>::template store<STREAM>(out + col, g);
     });
   }
 };
