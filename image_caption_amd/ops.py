@@ -450,12 +450,12 @@ def token_log_probs(logits, tokens, top_k=0, pad_token=-1):
     V, N, dev, shape, top_k = logits.shape[-1], tokens.numel(), logits.device, tokens.shape, int(top_k)
     if not 0 <= top_k <= min(V, _lib.MAX_ALTERNATIVES):
         raise ValueError("token_log_probs: top_k must be in 0 .. min(V, %d)" % _lib.MAX_ALTERNATIVES)
-    log_probs = torch.empty(shape, dtype=f32, device=dev)
-    entropy = torch.empty(shape, dtype=f32, device=dev)
-    stats = torch.empty(*shape, 2, dtype=f32, device=dev)
-    top_ids = torch.empty(*shape, top_k, dtype=i32, device=dev) if top_k else None
-    top_lp = torch.empty(*shape, top_k, dtype=f32, device=dev) if top_k else None
     x, t = _chk(logits, DTYPES, "logits", rows=True), _chk(tokens, i32, "tokens")
+    log_probs = torch.empty_like(tokens, dtype=f32)
+    entropy = torch.empty_like(log_probs)
+    stats = torch.empty((*shape, 2), dtype=f32, device=dev)
+    top_ids = torch.empty((*shape, top_k), dtype=i32, device=dev) if top_k else None
+    top_lp = torch.empty_like(top_ids, dtype=f32) if top_k else None
     if N:
         _call("icap_token_log_probs", x, DTYPES[logits.dtype], N, V, *_row_split(logits, "logits"), t,
               int(pad_token), top_k, log_probs.data_ptr(), entropy.data_ptr(), stats.data_ptr(),

@@ -1,6 +1,8 @@
 """Sequence generators of the sequence-level trainers (reference utils/agent_utils.py:30-284):
 the sampler and the beam-search baseline, same class names, constructor arguments and call
 signatures; tensors are torch tensors on the ROCm device."""
+from collections import namedtuple
+
 import torch
 
 from .. import ops
@@ -80,6 +82,52 @@ class SequenceSampler(object):
             samples.append(sample.reshape(-1, 1))
             dec_input = sample
         return torch.cat(samples, dim=-1).to(self.data_type)
+
+
+SequenceScores = namedtuple("SequenceScores", ("log_probs", "entropy", "top_ids", "top_log_probs",
+                                               "logits", "stats", "tokens"))
+
+
+class SequenceScorer(object):
+    """What the sequence-level trainers need of given sequences next (their policy-gradient steps are
+    utils/train_utils.py:397,432,476): __call__((features, sequences)) feeds the policy the
+    sequences' tokens and returns, for each token after the first, its log probability and the
+    entropy of the distribution it was drawn from - SequenceScores of [B, T-1] float32, zeros at
+    pad_token; with top_k also the best alternatives [B, T-1, top_k].  `grad` takes gradients of the
+    two back to the logits, [B, T-1, V]."""
+
+    def __init__(self, action_network, pad_token=0, top_k=0):
+        self.action_network = action_network
+        self.pad_token = pad_token
+        self.top_k = top_k
+
+    def __call__(self, inputs, **kwargs):
+        features, sequences = inputs
+        batch_size, steps = sequences.shape
+        if steps < 2:
+            raise ValueError("SequenceScorer: sequences need a token after the first")
+        sequences = sequences.to(torch.int32)
+        state = self.action_network.reset_state(sequences, {"features": features}, **kwargs)
+        logits = []
+        for time_step in range(1, steps):
+            predictions, state = self.action_network(
+                (sequences[:, time_step - 1].contiguous(), {"features": features}, state), **kwargs)
+            logits.append(predictions.reshape(batch_size, -1))
+        logits = torch.stack(logits)                                 # time first, as they came
+        tokens = sequences[:, 1:].t().contiguous()
+        log_probs, entropy, stats, top_ids, top_log_probs = ops.token_log_probs(
+            logits, tokens, top_k=self.top_k, pad_token=self.pad_token)
+        first = lambda t: None if t is None else t.transpose(0, 1)   # noqa: E731  (batch first)
+        return SequenceScores(log_probs.t(), entropy.t(), first(top_ids), first(top_log_probs),
+                              first(logits), first(stats), tokens.t())
+
+    def grad(self, scores, grad_log_probs=None, grad_entropy=None):
+        """Gradient to scores.logits of sum(grad_log_probs * log_probs + grad_entropy * entropy)."""
+        time_first = lambda t: None if t is None else t.transpose(0, 1).contiguous()   # noqa: E731
+        return ops.token_log_probs_grad(
+            time_first(scores.logits), time_first(scores.tokens), time_first(scores.stats),
+            time_first(scores.entropy), time_first(grad_log_probs), time_first(grad_entropy),
+            pad_token=self.pad_token).transpose(0, 1)
 
 
 class BaselineSequeneBeamSearcher(object):
