@@ -317,7 +317,9 @@ template <int DTYPE, bool STREAM>
 __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs p) {
   typedef Elem<DTYPE> E;
   typedef typename E::type type;
-  const int row = blockIdx.x / p.shares, share = blockIdx.x % p.shares, tid = threadIdx.x;
+  const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  const int row = (int)(block / p.shares), share = (int)(block % p.shares), tid = threadIdx.x;
+  if (row >= p.N) return;
   const int token = p.tokens[row];
   const type* x = (const type*)p.logits + p.view.at(row);
   type* g = (type*)p.out + p.out_view.at(row);
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p)
   }
 }
 
-constexpr long long kMostBlocks = (1LL << 32) / 1024 - 1;      // a launch counts 2^32 lanes along x
+constexpr int kMostRows = 1 << 30;      // workgroup numbers stay within 31 bits, the last row of them unfilled
 
 dim3 row_grid(int N) {
   const int x = N < 65536 ? N : 65536;
@@ -522,7 +524,8 @@ int check_rows(const char* what, int dtype, int N, int V, const RowView& v) {
   ICAP_REQUIRE(dtype == ICAP_DTYPE_F32 || dtype == ICAP_DTYPE_BF16 || dtype == ICAP_DTYPE_F16,
                "%s: unknown dtype %d", what, dtype);
   ICAP_REQUIRE(N > 0 && V > 0, "%s: bad shape", what);
-  ICAP_REQUIRE(V <= 0x7fff0000, "%s: V too large", what);
+  if (N > kMostRows || V > kMostRows)
+    return fail(ICAP_ERR_UNSUPPORTED, "%s: N and V go up to %d", what, kMostRows);
   ICAP_REQUIRE(v.inner > 0 && v.ld >= 0 && v.ld_outer >= 0, "%s: bad strides", what);
   return ICAP_OK;
 }
@@ -654,11 +657,11 @@ int icap_token_log_probs_grad(const void* logits, int dtype, int N, int V, int r
   ScoreGradArgs a{logits, view, tokens, N, V, pad_token, stats, entropy, grad_log_probs, grad_entropy, dlogits, out,
                   std::max(1, ceil_div(V / (dtype == ICAP_DTYPE_F32 ? 4 : 8), NT * kGradPieces))};
   const long long blocks = (long long)N * a.shares;
-  if (blocks > kMostBlocks)
+  if (blocks > kMostRows)
     return fail(ICAP_ERR_UNSUPPORTED, "token_log_probs_grad: %d rows of %d are too many for one call", N, V);
   const bool streamed = stream_writes(row_bytes(dtype, N, V));
 #define LAUNCH_S(D, S)                                                                          \
-  hipLaunchKernelGGL((token_log_probs_grad_kernel<D, S>), dim3((unsigned)blocks), dim3(NT), 0,  \
+  hipLaunchKernelGGL((token_log_probs_grad_kernel<D, S>), row_grid((int)blocks), dim3(NT), 0,  \
                      (hipStream_t)stream, a)
 #define LAUNCH(D) do { if (streamed) LAUNCH_S(D, true); else LAUNCH_S(D, false); } while (0)
   ICAP_BY_DTYPE(dtype, LAUNCH);

@@ -112,7 +112,7 @@ def test_scores_and_gradient_of_large_vocabularies(kind, V, N):
     _check_score_grad(x, tokens, out[2], out[1], g_lp, g_h, kind=kind)
 
 
-@pytest.mark.parametrize("kind,N,V", [("f32", 300, 1000), ("bf16", 2100, 257), ("f16", 600, 2000), ("f32", 5000, 33)])
+@pytest.mark.parametrize("kind,N,V", [("f32", 1400, 3000), ("bf16", 800, 5000), ("f16", 2699, 3000), ("f32", 300, 1000), ("bf16", 2100, 257), ("f16", 600, 2000), ("f32", 5000, 33)])
 def test_scores_of_many_rows(kind, N, V):
     rng = np.random.default_rng(N)
     x = _logits(rng, N, V, kind)
@@ -128,7 +128,7 @@ def test_masked_logits(kind, V):
     """-inf and the type's lowest value among the logits, rows of nothing else, NaN and +inf, rows of
     the padding token that hold NaN, tokens outside the vocabulary."""
     rng = np.random.default_rng(V)
-    x = (rng.standard_normal((14, V)) * 2).astype(np.float32)
+    x = (rng.standard_normal((17, V)) * 2).astype(np.float32)
     x[0, rng.random(V) < 0.5] = -np.inf
     x[0, V // 2] = 1.0
     x[1, rng.random(V) < 0.5] = LOWEST[kind]
@@ -146,21 +146,24 @@ def test_masked_logits(kind, V):
     x[12] = LOWEST[kind]
     x[12, 1] = -np.inf
     x[13] *= 30 if kind == "f16" else 1e4
-    tokens = np.array([V // 2, 1, 0, 2, V - 1, 1, 1, 0, 3, 4, 0, V, 1, 2])
+    x[14] *= 1 if kind == "f16" else 1e9          # rate * x rounds off what tells the elements apart
+    x[15] *= 1 if kind == "f16" else 1e30
+    x[16] -= 1 if kind == "f16" else 1e8
+    tokens = np.array([V // 2, 1, 0, 2, V - 1, 1, 1, 0, 3, 4, 0, V, 1, 2, 1, 2, 3])
     tokens[2] = 1
     tokens[10] = 4
     pad = 0
     xd = _dev(x, kind)
     out = _check_score(xd, tokens, pad=pad, k=min(V, 9))
-    g = np.full(14, 0.5)
+    g = np.full(17, 0.5)
     _check_score_grad(xd, tokens, out[2], out[1], g, -g, pad=pad, kind=kind)
     for bad in (-1, -7, V, V + 5, 2 ** 31 - 1, -2 ** 31):
-        t = np.full(14, bad)
+        t = np.full(17, bad)
         t[7] = pad
         out = _check_score(xd, t, pad=pad, k=1)
         _check_score_grad(xd, t, out[2], out[1], g, None, pad=pad, kind=kind)
         _check_score_grad(xd, t, out[2], out[1], None, g, pad=pad, kind=kind)
-    zero = np.zeros(14)
+    zero = np.zeros(17)
     zero[0] = 1.0                                 # gradients of zero leave rows of NaN at zero
     _check_score_grad(xd, tokens, out[2], out[1], zero, zero * 0, pad=pad, kind=kind)
 
@@ -333,11 +336,66 @@ def test_distillation(kind, V):
         _check_distill(x, tl, ti, tau, None, kind, "N=%d K=%d" % (N, K))
 
 
+@pytest.mark.parametrize("kind,V", [("f32", 5), ("f32", 1000), ("f32", 2047), ("f32", 4001), ("f32", 9000), ("f32", 10243),
+                                    ("f32", 28675), ("f32", 30000), ("bf16", 2049), ("bf16", 4095), ("bf16", 8191),
+                                    ("f16", 20481), ("bf16", 53247), ("f16", 53255), ("bf16", 60000)])
+def test_distillation_of_many_rows(kind, V):
+    """Every division of a row over waves and registers that a batch of over 512 rows takes."""
+    rng = np.random.default_rng(V)
+    N, K = 520, min(V, 20)
+    x = _logits(rng, N, V, kind)
+    x[::7, ::3] = float("-inf")
+    ti = rng.integers(0, V, (N, K))
+    ti[::7] = ti[::7] // 3 * 3 + 1 if V > 5 else 1
+    ti = np.minimum(ti, V - 1)
+    ti[rng.random(N) < 0.2] = -1
+    _check_distill(x, _logits(rng, N, K, "f32"), ti, 2.0, rng.standard_normal(N), kind)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_streams_past_the_caches_give_the_same_bits(in_place):
+    """Calls so large that they go past the caches, against the same rows in smaller calls."""
+    from image_caption_amd import ops
+    g = torch.Generator(device=dev())
+    g.manual_seed(1)
+    x = torch.randn(5500, 20000, device=dev(), generator=g)
+    tokens = torch.randint(0, 20000, (5500,), device=dev(), generator=g, dtype=torch.int32)
+    for k in (0, 5):
+        whole = ops.token_log_probs(x, tokens, top_k=k)
+        for r in (slice(0, 2750), slice(2750, 5500)):
+            part = ops.token_log_probs(x[r], tokens[r], top_k=k)
+            assert all(torch.equal(a[r], b) for a, b in zip(whole, part) if b is not None)
+    lp, h, stats = whole[:3]
+    a, b = (torch.randn(5500, device=dev(), generator=g) for _ in range(2))
+    ti = torch.randint(-1, 20000, (5500, 30), device=dev(), generator=g, dtype=torch.int32)
+    tl = torch.randn(5500, 30, device=dev(), generator=g)
+    parts = [slice(i, i + 1100) for i in range(0, 5500, 1100)]
+    small = torch.cat([ops.token_log_probs_grad(x[r], tokens[r], stats[r], h[r], a[r], b[r]) for r in parts])
+    y = x.clone() if in_place else x
+    assert torch.equal(ops.token_log_probs_grad(y, tokens, stats, h, a, b, out=y if in_place else None), small)
+    pairs = [ops.distill_loss(x[r], tl[r], ti[r], 1.5, a[r]) for r in parts]
+    y = x.clone() if in_place else x
+    loss, grad = ops.distill_loss(y, tl, ti, 1.5, a, out=y if in_place else None)
+    assert torch.equal(loss, torch.cat([p[0] for p in pairs])) and torch.equal(grad, torch.cat([p[1] for p in pairs]))
+    del x, y, small, grad, pairs
+    table = torch.randn(3000, 256, device=dev(), generator=g)
+    ids = torch.randint(-2, 3002, (120000,), device=dev(), generator=g, dtype=torch.int32)
+    rows = ops.embedding_scaled(table, ids, scale=3.0, pad_token=7)
+    assert torch.equal(rows, torch.cat([ops.embedding_scaled(table, i, scale=3.0, pad_token=7) for i in ids.split(60000)]))
+    got = ops.embedding_grad(rows, ids, 3000, scale=0.5, pad_token=7)
+    keep = (ids >= 0) & (ids < 3000) & (ids != 7)
+    want = torch.zeros(3000, 256, device=dev(), dtype=torch.float64)
+    want.index_add_(0, ids[keep].long(), rows[keep].double())
+    size = torch.zeros_like(want).index_add_(0, ids[keep].long(), rows[keep].double().abs())
+    count = torch.bincount(ids[keep].long(), minlength=3000).double()[:, None]
+    assert ((got.double() - 0.5 * want).abs() <= U * (count + 2) * size).all()
+
+
 @pytest.mark.parametrize("kind", sorted(TYPES))
 @pytest.mark.parametrize("V", [50, 3000, 70001])
 def test_distillation_entries_that_are_absent_double_or_wrong(kind, V):
     rng = np.random.default_rng(V)
-    K, N = 6, 17
+    K, N = 6, 20
     x = (rng.standard_normal((N, V)) * 2).astype(np.float32)
     ti = np.stack([rng.permutation(V)[:K] for _ in range(N)])
     tl = (rng.standard_normal((N, K)) * 2).astype(np.float32)
@@ -361,6 +419,10 @@ def test_distillation_entries_that_are_absent_double_or_wrong(kind, V):
     ti[14] = -1
     tl[15] = LOWEST["f16"]
     x[16] = LOWEST[kind]
+    if kind != "f16":
+        x[17] *= 1e9
+        x[18] *= 1e30
+        x[19] -= 1e8
     for g in (np.ones(N), np.where(np.arange(N) % 2, 0.0, -1.5), None):
         want_nan = g is not None
         _check_distill_rows(_dev(x, kind), _dev(tl), ti, 2.0, g, kind, skip_grad=[13] if want_nan else [])
@@ -477,6 +539,11 @@ def test_embedding_gradient_of_padding_that_holds_nan_and_of_nothing():
     want = torch.zeros(5, 8, device=dev())
     want[1], want[2] = 2.0, 1.0
     assert torch.equal(got, want)
+    from image_caption_amd import _lib
+    out, ws = torch.ones(5, 8, device=dev()), torch.empty(4096, dtype=torch.uint8, device=dev())
+    _lib.call("icap_embedding_grad", grad.data_ptr(), 0, grad.data_ptr(), out.data_ptr(), 0, 5, 8, 1.0, -1,
+              ws.data_ptr(), 4096, torch.cuda.current_stream().cuda_stream)      # no tokens at all
+    assert not out.any()
     none = ops.embedding_grad(torch.zeros(0, 8, device=dev()), _ids(np.zeros(0)), 5)
     assert tuple(none.shape) == (5, 8) and not none.any()
 

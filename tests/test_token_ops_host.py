@@ -46,6 +46,14 @@ def test_limits_of_alternatives_and_teacher_entries():
     mod, lib = _lib()
     assert _score(lib, V=100, ld=100, k=mod.MAX_ALTERNATIVES + 1, ids=P, top=P) == -3
     assert _distill(lib, K=mod.MAX_TEACHER_LOGITS + 1) == -3
+    most = 1 << 30
+    assert _score(lib, N=most + 1, V=1, ld=1, inner=most + 1) == -3
+    assert _score_grad(lib, N=most + 1, V=1, ld=1, inner=most + 1, out_ld=1) == -3
+    assert _score_grad(lib, N=most, V=8192, ld=8192, inner=most, out_ld=8192) == -3
+    assert _distill(lib, N=most + 1, V=1, ld=1, inner=most + 1, out_ld=1) == -3
+    assert _score(lib, N=1, V=most + 1, ld=most + 1) == -3
+    assert lib.icap_embedding_scaled(P, 0, P, P, (1 << 25) + 1, 8, 8, 1.0, -1, None) == -3
+    assert lib.icap_embedding_grad(P, 0, P, P, 8, (1 << 25) + 1, 8, 1.0, -1, P, 1 << 40, None) == -3
 
 
 @pytest.mark.parametrize("bad", [dict(logits=None), dict(tokens=None), dict(st=None), dict(h=None), dict(out=None),
