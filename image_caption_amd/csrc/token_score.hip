@@ -382,10 +382,14 @@ struct DistillArgs {
   RowView out_view;
 };
 
-__device__ __forceinline__ float load_typed(const void* p, int dtype, size_t i) {
-  if (dtype == ICAP_DTYPE_F32) return ((const float*)p)[i];
-  if (dtype == ICAP_DTYPE_BF16) return (float)((const __bf16*)p)[i];
-  return (float)((const _Float16*)p)[i];
+// An element's bits, and what they stand for: apart, so that a load can stay in flight meanwhile.
+__device__ __forceinline__ uint32_t load_bits(const void* p, int dtype, size_t i) {
+  return dtype == ICAP_DTYPE_F32 ? ((const uint32_t*)p)[i] : ((const uint16_t*)p)[i];
+}
+__device__ __forceinline__ float bits_value(uint32_t bits, int dtype) {
+  if (dtype == ICAP_DTYPE_F32) return __uint_as_float(bits);
+  if (dtype == ICAP_DTYPE_BF16) return __uint_as_float(bits << 16);
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
 // Only what goes through LDS is ordered: loads and stores of device memory stay in flight.
@@ -398,13 +402,15 @@ __device__ __forceinline__ void lds_barrier() {
 // loss = tau^2 sum_k q_k (log q_k - log p[id_k]),  q = soft-max of the teacher's K logits at tau,
 // p = soft-max of the row at tau;   d loss / d x_j = tau (p_j - sum over k with id_k = j of q_k)
 //
-// A workgroup reads a row into registers, sums it, and writes the gradient from there; the row is
-// read while the first wave takes the teacher's entries along, and one barrier hands their q and
-// the waves' sums round.  (A workgroup that goes through several rows and reads the next one into a
+// A workgroup reads a row into registers, sums it, and writes the gradient from there; one barrier
+// hands the waves' sums and the teacher's q round.  (A workgroup that goes through several rows and reads the next one into a
 // second set of registers was slower, 158 against 122 us for 2560 rows of 50000 in bf16: the
 // registers cost it half of its neighbours, which hide the same latency.)
+//
+// The second launch bound holds a thread to the registers that 8 waves a SIMD leave (7 and 6 for 10 and
+// 13 pieces); without it 4000 rows of 20000 in fp32 take 161 instead of 120 us.
 template <int DTYPE, int WAVES, int NV, bool STREAM>
-__global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p) {
+__global__ __launch_bounds__(WAVES * 64, NV == 13 ? 6 : NV == 10 ? 7 : 8) void distill_loss_kernel(DistillArgs p) {
   typedef Elem<DTYPE> E;
   typedef typename E::type type;
   __shared__ RowStats s_part[WAVES];
@@ -417,29 +423,44 @@ __global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p)
   const float inv_tau = 1.f / p.tau, rate = kLog2e * inv_tau;
   type* g = p.out ? (type*)p.out + p.out_view.at(row) : nullptr;
   // every wave looks for itself whether the teacher has an entry
-  bool any = false;
-  for (int k = lane; k < p.K; k += 64) any |= p.t_ids[(size_t)row * p.K + k] != -1;
+  const int32_t* ids = p.t_ids + (size_t)row * p.K;
+  const int id0 = lane < p.K ? ids[lane] : -1;
+  bool any = id0 != -1;
+  for (int k = lane + 64; k < p.K; k += 64) any |= ids[k] != -1;
   if (!__any(any)) {
     if (tid == 0) p.loss[row] = 0.f;
     if (g) write_zeros<DTYPE, WAVES, STREAM>(g, p.V);
     return;
   }
+  // The last wave (its share of the row is the shortest) sees to the teacher's entries.  It asks for
+  // the first 64 before the row, whose sums they then do not delay.
+  const type* x = (const type*)p.logits + p.view.at(row);
+  const bool teaches = wave == WAVES - 1;
+  uint32_t t0 = 0, x0 = 0;
+  if (teaches && id0 != -1) {
+    t0 = load_bits(p.t_logits, p.t_dtype, (size_t)row * p.K + lane);
+    if ((unsigned)id0 < (unsigned)p.V) x0 = load_bits(x, DTYPE, id0);
+  }
   Row<DTYPE, WAVES, NV, STREAM> data;
-  data.open((const type*)p.logits + p.view.at(row), p.V);
+  data.open(x, p.V);
   const float coef = g ? p.g_loss[row] * p.tau : 0.f;
-  if (wave == 0) {      // (a lane reads back only what it wrote itself)
+  RowStats part = row_stats_lanes<64>(data.sums(rate), rate);
+  if (lane == 0) s_part[wave] = part;
+  if (teaches) {        // (a lane reads back only what it wrote itself)
     bool bad = false, entries = false;
     float top = -INFINITY;
 #pragma unroll 1
     for (int k = lane; k < p.K; k += 64) {
-      const int id = p.t_ids[(size_t)row * p.K + k];
+      const int id = k < 64 ? id0 : ids[k];
       const bool in = (unsigned)id < (unsigned)p.V;
-      const float t = id == -1 ? -INFINITY : load_typed(p.t_logits, p.t_dtype, (size_t)row * p.K + k);
+      float t = -INFINITY, xk = 0.f;
+      if (id != -1) t = bits_value(k < 64 ? t0 : load_bits(p.t_logits, p.t_dtype, (size_t)row * p.K + k), p.t_dtype);
+      if (in) xk = bits_value(k < 64 ? x0 : load_bits(x, DTYPE, id), DTYPE);
       bad |= id != -1 && !in;
       entries |= !(t == -INFINITY);
       top = fmaxf(top, t);
       s_id[k] = in ? id : -1;
-      s_x[k] = in ? E::up(data.x[id]) : 0.f;
+      s_x[k] = xk;
       s_log_q[k] = t;
     }
     bad = __any(bad);
@@ -462,8 +483,6 @@ __global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p)
     }
     if (lane == 0) s_state = (entries ? 1 : 0) | (bad ? 2 : 0);
   }
-  RowStats part = row_stats_lanes<64>(data.sums(rate), rate);
-  if (lane == 0) s_part[wave] = part;
   lds_barrier();
   const RowResult r =
       row_result(row_stats_lanes<WAVES>(s_part[lane & (WAVES - 1)], rate), rate, [&](float m) {
@@ -476,7 +495,7 @@ __global__ __launch_bounds__(WAVES * 64) void distill_loss_kernel(DistillArgs p)
         return row_stats_lanes<WAVES>(s_part[lane & (WAVES - 1)], rate);
       });
   const bool bad = s_state & 2, entries = s_state;
-  if (wave == 0) {
+  if (teaches) {
     float sum = 0.f;
 #pragma unroll 1
     for (int k = lane; k < p.K; k += 64) {
@@ -556,11 +575,12 @@ int waves_per_row(int dtype, int N, int V) {
 // Waves for a row and pieces a thread holds: as few waves as keep some 10 pieces a thread or less, more
 // where two or three such rows still fit a compute unit's registers, and longer rows read twice.
 // Few rows go to large workgroups: their time is that of one row.  Measured, us, with one read and one
-// write of the logits at the rate of a copy in brackets: 40000 rows of 2000 in fp32 140 (121) by 2
-// waves of 4, 156 by 1 of 8, 162 by 4 of 4; 10240 of 10000 in fp32 162 (155) by 8 of 5, 166 by 4 of 10; in
-// bf16 94 (77) by 4 of 10, 117 by 8 of 5; 2560 of 50000 in bf16 108 (97) by 8 of 13, 115 by 16 of 7, 113 by
-// 4 of 25; 4000 of 20000 in fp32 121 (121) by 16 of 7, 128 by 8 of 13; 2048 of 50000 in fp32 189 (155)
-// read twice, 201 by 16 of 13.
+// write of the logits at the rate of a copy in brackets: 40000 rows of 2000 in fp32 130 (121) by 2
+// waves of 4, and before the teacher's entries were asked for ahead of the row 140 against 156 by 1 of 8
+// and 162 by 4 of 4; 10240 of 10000 in fp32 149 (155) by 8 of 5, 161 then against 166 by 4 of 10; in bf16
+// 81 (77) by 4 of 10, 87 then against 117 by 8 of 5; 2560 of 50000 in bf16 112 (97) by 8 of 13, 108 then
+// against 115 by 16 of 7 and 113 by 4 of 25; 4000 of 20000 in fp32 120 (121) by 16 of 7, 121 then against
+// 128 by 8 of 13; 2048 of 50000 in fp32 189 (155) read twice, 201 then by 16 of 13.
 struct RowShape {
   int waves, held;
 };
