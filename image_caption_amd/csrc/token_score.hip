@@ -36,18 +36,18 @@ struct TopScratch {                // of one wave
   unsigned long long key[kNotes];
 };
 
-// A value that at least k of the lanes reach, close below the k-th largest of their 64: the bits of
-// its order from the top down, until exactly k lanes reach it or 12 bits of the mantissa are known.
+// A value that at least k of the lanes reach, the k-th largest of their 64 or close below it: the bits
+// of its order from the top down, until exactly k lanes reach it.  Lanes that tie have it exact.
 __device__ __forceinline__ float kth_of_lanes(float v, int k) {
   const uint32_t mine = order_of(v);
   uint32_t bound = 0;
-  for (int bit = 31; bit >= 12; --bit) {
+  for (int bit = 31; bit >= 0; --bit) {
     const uint32_t next = bound | (1u << bit);
     const int reach = __popcll(__ballot(mine >= next));
     if (reach >= k) bound = next;
     if (reach == k) break;
   }
-  return fmaxf(order_value(bound), kLowest);
+  return fmaxf(order_value(bound), -INFINITY);      // (below -inf in the order: a NaN's bits)
 }
 
 // One wave's share of a row: pieces [from, to) of kVec elements, read once in batches of kBatch a
@@ -59,6 +59,7 @@ struct Share {
   static constexpr int kBatch = kBatchElems / E::kVec;
   const type* x;
   int from, to, lane;
+  int end;                     // columns of the share are [from * kVec, end)
   int tail_col;                // -1: no single element here
   float tail;
 
@@ -73,7 +74,10 @@ struct Share {
 // The share's statistics and, with TOP, its k best columns as ranked keys in best[0 .. k) (0: none
 // left).  While the share is read the wave keeps a bound that at least k elements have reached - the
 // k-th largest of the lanes' maxima so far, renewed after 1, 2, 4, 8 ... batches - and notes the
-// batches of a lane that reach it; in the end some k to 2k of them are read again.
+// batches of a lane that reach it; in the end some k to 2k of them are read again.  Batches come in
+// the order of their columns, so what only equals a bound that stood before its batch has k better
+// or equal elements at lower columns and is not noted: rows of equal logits (masked to the lowest
+// value, or not trained yet) note one batch.
 template <int DTYPE, bool TOP, bool STREAM>
 __device__ __forceinline__ RowStats share_scan(const Share<DTYPE, STREAM>& sh, float rate, int k, TopScratch& s,
                                                unsigned long long* best) {
@@ -82,52 +86,57 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE, STREAM>& sh, f
   const unsigned long long lower = (1ull << sh.lane) - 1;
   RowStats a = row_stats_empty();
   const int batches = (sh.to - sh.from + kBatch * 64 - 1) / (kBatch * 64);
-  float bound = kLowest;
+  float lane_top = -INFINITY, bound = -INFINITY, stood = -INFINITY;
   int notes = 0, renew = 0;
   bool full = false;
   // a new bound, and of the notes only those that reach it
   auto squeeze = [&]() {
-    bound = kth_of_lanes(a.m, k);
+    bound = kth_of_lanes(lane_top, k);
     int kept = 0;
     wave_sync();
     for (int i0 = 0; i0 < notes; i0 += 64) {
       const int i = i0 + sh.lane;
-      const float m = i < notes ? s.note_max[i] : -INFINITY;
-      const int what = i < notes ? s.note[i] : 0;
-      const unsigned long long keep = __ballot(m >= bound);
+      const bool there = i < notes;
+      const float m = there ? s.note_max[i] : 0.f;
+      const int what = there ? s.note[i] : 0;
+      const bool keep = there && m >= bound;
+      const unsigned long long mask = __ballot(keep);
       wave_sync();
-      if (m >= bound) {
-        const int at = kept + __popcll(keep & lower);
+      if (keep) {
+        const int at = kept + __popcll(mask & lower);
         s.note_max[at] = m;
         s.note[at] = what;
       }
-      kept += __popcll(keep);
+      kept += __popcll(mask);
       wave_sync();
     }
     notes = kept;
   };
   auto note = [&](float m, int what) {
-    unsigned long long hit = __ballot(m >= bound);
-    if (!hit || full) return;
-    if (notes + __popcll(hit) > kNotes) {
-      squeeze();
-      hit = __ballot(m >= bound);
-      full = notes + __popcll(hit) > kNotes;
-      if (full) return;
+    unsigned long long hit = __ballot(m >= bound && m > stood);
+    if (hit && !full) {
+      if (notes + __popcll(hit) > kNotes) {
+        squeeze();
+        hit = __ballot(m >= bound && m > stood);
+        full = notes + __popcll(hit) > kNotes;
+      }
+      if (!full) {
+        if ((hit >> sh.lane) & 1) {
+          const int at = notes + __popcll(hit & lower);
+          s.note_max[at] = m;
+          s.note[at] = what;
+        }
+        notes += __popcll(hit);
+      }
     }
-    if (m >= bound) {
-      const int at = notes + __popcll(hit & lower);
-      s.note_max[at] = m;
-      s.note[at] = what;
-    }
-    notes += __popcll(hit);
+    stood = bound;
   };
   for (int b = 0; b < batches; ++b) {
     u32x4 r[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) r[j] = sh.read(sh.piece(b, j));
     float v[kBatch][E::kVec];
-    float top = kLowest;
+    float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       E::unpack(r[j], v[j]);
@@ -140,8 +149,9 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE, STREAM>& sh, f
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) row_stats_add(a.s, a.w, v[j], rate, c);
     if constexpr (TOP) {
+      lane_top = fmaxf(lane_top, top);
       if (b == renew) {
-        bound = kth_of_lanes(a.m, k);
+        bound = kth_of_lanes(lane_top, k);
         renew = 2 * b + 1;
       }
       note(top, b * 64 + sh.lane);
@@ -153,51 +163,101 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE, STREAM>& sh, f
   a.m = m;
   row_stats_add(a.s, a.w, tail, rate, c);
   if constexpr (TOP) {
+    lane_top = fmaxf(lane_top, sh.tail);
     if (__any(sh.tail_col >= 0)) note(sh.tail_col >= 0 ? sh.tail : -INFINITY, -1 - sh.tail_col);
     squeeze();
     if (sh.lane < k) best[sh.lane] = 0;
-    int count = 0;
-    auto candidate = [&](bool is, float v, int col) {
-      const unsigned long long hit = __ballot(is);
-      if (!hit) return;
-      const int at = count + __popcll(hit & lower);
-      if (is && at < kNotes) s.key[at] = rank_key(v, col);
-      count += __popcll(hit);
-    };
-    if (!full)
+    // f(value, column) for the elements of the noted batches, all lanes together (NaN: none here)
+    auto each_noted = [&](auto f) {
       for (int t0 = 0; t0 < notes * kBatch; t0 += 64) {
         const int t = t0 + sh.lane;
-        const int what = t < notes * kBatch ? s.note[t / kBatch] : 0;
+        const bool there = t < notes * kBatch;
+        const int what = there ? s.note[t / kBatch] : 0;
         const bool single = what < 0;      // one element behind the last piece
         const int i = sh.from + (what / 64 * kBatch + t % kBatch) * 64 + what % 64;
-        const bool there = t < notes * kBatch && !single && i < sh.to;
         float v[E::kVec];
 #pragma unroll
         for (int e = 0; e < E::kVec; ++e) v[e] = NAN;
-        if (there) E::unpack(*reinterpret_cast<const u32x4_any*>(sh.x + (size_t)i * E::kVec), v);
-        if (t < notes * kBatch && single && t % kBatch == 0) v[0] = E::up(sh.x[-1 - what]);
+        if (there && !single && i < sh.to)
+          E::unpack(*reinterpret_cast<const u32x4_any*>(sh.x + (size_t)i * E::kVec), v);
+        if (there && single && t % kBatch == 0) v[0] = E::up(sh.x[-1 - what]);
 #pragma unroll
-        for (int e = 0; e < E::kVec; ++e) candidate(v[e] >= bound, v[e], single ? -1 - what : i * E::kVec + e);
+        for (int e = 0; e < E::kVec; ++e) f(v[e], single ? -1 - what : i * E::kVec + e);
       }
-    wave_sync();
-    if (!full && count >= k && count <= kNotes) {
+    };
+    // those that reach the bound, or if they are too many, as in rows of equal logits, or the bound is
+    // -inf, those over it
+    int count = kNotes + 1;
+    for (int over = bound == -INFINITY; over < 2 && !full && count > kNotes; ++over) {
+      count = 0;
+      each_noted([&](float v, int col) {
+        const bool is = over ? v > bound : v >= bound;
+        const unsigned long long hit = __ballot(is);
+        if (!hit) return;
+        const int at = count + __popcll(hit & lower);
+        if (is && at < kNotes) s.key[at] = rank_key(v, col);
+        count += __popcll(hit);
+      });
+      wave_sync();
+    }
+    if (!full && count <= kNotes) {
       for (int i = sh.lane; i < count; i += 64) {
         const unsigned long long key = s.key[i];
         int rank = 0;
         for (int j = 0; j < count; ++j) rank += s.key[j] > key;
         if (rank < k) best[rank] = key;
       }
+      if (count < k && bound == -INFINITY) {
+        // the lowest of the other columns follow, all of which lie within the share's first 64
+        const int col = sh.from * E::kVec + sh.lane;
+        const bool other = col < sh.end && !(E::up(sh.x[min(col, sh.end - 1)]) > -INFINITY);
+        const int at = count + __popcll(__ballot(other) & lower);
+        if (other && at < k) best[at] = rank_key(-INFINITY, col);
+      } else if (count < k) {
+        // those that equal the bound follow, in the order of their columns
+        int at = count, last = -1;
+        for (int i = 0; i < notes && at < k; ++i) {
+          const int what = __builtin_amdgcn_readfirstlane(s.note[i]);
+          if (what < 0) {
+            const bool equal = sh.tail_col >= 0 && sh.tail == bound;
+            const int slot = at + __popcll(__ballot(equal) & lower);
+            if (equal && slot < k) best[slot] = rank_key(bound, sh.tail_col);
+            break;
+          }
+          if (what / 64 == last) continue;
+          last = what / 64;
+          for (int j = 0; j < kBatch && at < k; ++j) {
+            float v[E::kVec];
+            E::unpack(sh.read(sh.piece(last, j)), v);
+            int slot = at;
+#pragma unroll
+            for (int e = 0; e < E::kVec; ++e) {
+              const unsigned long long hit = __ballot(v[e] == bound);
+              slot += __popcll(hit & lower);
+              at += __popcll(hit);
+            }
+#pragma unroll
+            for (int e = 0; e < E::kVec; ++e)
+              if (v[e] == bound) {
+                if (slot < k) best[slot] = rank_key(bound, sh.piece(last, j) * E::kVec + e);
+                ++slot;
+              }
+          }
+        }
+      }
     } else {
-      // many elements that tie with the bound, or fewer than k over -inf: a round for each
+      // more elements over the bound than fit: a round for each, over the noted batches or,
+      // if those did not fit either, over the share
       unsigned long long below = ~0ull;
       for (int r = 0; r < k; ++r) {
         unsigned long long key = 0;
-        auto look = [&](int col) {
-          const unsigned long long q = rank_key(E::up(sh.x[col]), col);
-          if (q < below && q > key) key = q;
+        auto look = [&](float v, int col) {
+          const unsigned long long q = rank_key(v, col);
+          if (v >= bound && q < below && q > key) key = q;
         };
-        for (int col = sh.from * E::kVec + sh.lane; col < sh.to * E::kVec; col += 64) look(col);
-        if (sh.tail_col >= 0) look(sh.tail_col);
+        if (!full) each_noted(look);
+        else
+          for (int col = sh.from * E::kVec + sh.lane; col < sh.end; col += 64) look(E::up(sh.x[col]), col);
         for (int d = 32; d > 0; d >>= 1) key = max(key, (unsigned long long)__shfl_xor(key, d, 64));
         below = key;
         if (sh.lane == 0) best[r] = key;
@@ -211,6 +271,12 @@ __device__ __forceinline__ RowStats share_scan(const Share<DTYPE, STREAM>& sh, f
 // P waves to a row, 4 / P rows to a workgroup (P = 1, 2) or one (P = 4, 8).  The waves of a row
 // meet once, when each has its share's statistics and its k best columns in LDS; the first joins
 // them.  Rows alone in a wave wait for nobody.
+//
+// Bound by one read of the logits: 10240 rows of 10000 in fp32, a quarter of them padding, 53 us (5.8
+// TB/s), 2560 rows of 50001 in bf16 with 16 alternatives 57 us (4.5 TB/s; without alternatives 43 us,
+// the bound and the notes are vector instructions).  Rows that are masked but for a few columns
+// cost the same within a fifth (few of 50001 bf16 columns left over the lowest value 62 us, nothing
+// but equal logits 58); those whose every logit is past 2^24 are read twice (106 us).
 template <int DTYPE, int P, bool TOP, bool STREAM>
 __global__ __launch_bounds__((P < 4 ? 4 : P) * 64, 8) void token_log_probs_kernel(ScoreArgs p) {
   typedef Elem<DTYPE> E;
@@ -228,13 +294,14 @@ __global__ __launch_bounds__((P < 4 ? 4 : P) * 64, 8) void token_log_probs_kerne
   const bool scored = live && token != p.pad;
   if (scored) {
     const int pieces = p.V / E::kVec;
-    // shares of whole batches
+    // shares of whole waves' pieces
     const int each = ((pieces + P - 1) / P + 63) / 64 * 64;
     Share<DTYPE, STREAM> sh;
     sh.x = x;
     sh.from = min(pieces, part * each);
     sh.to = min(pieces, sh.from + each);
     sh.lane = lane;
+    sh.end = part == P - 1 ? p.V : sh.to * E::kVec;
     const int tail_col = pieces * E::kVec + lane;
     sh.tail_col = part == P - 1 && tail_col < p.V ? tail_col : -1;
     sh.tail = sh.tail_col >= 0 ? E::up(x[tail_col]) : -INFINITY;
@@ -263,7 +330,16 @@ __global__ __launch_bounds__((P < 4 ? 4 : P) * 64, 8) void token_log_probs_kerne
   }
   const RowResult r = row_result(a, kLog2e, [&](float m) {
     RowStats f = {m, 0.f, 0.f};
-    for (int c = lane; c < p.V; c += 64) row_stats_add_far(f, E::up(x[c]), kLog2e);
+    const int pieces = p.V / E::kVec;
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += 64) {
+      float v[E::kVec];
+      E::unpack(load16<false>(x + (size_t)i * E::kVec), v);
+#pragma unroll
+      for (int e = 0; e < E::kVec; ++e) row_stats_add_far(f, v[e], kLog2e);
+    }
+    const int tail = pieces * E::kVec + lane;
+    if (tail < p.V) row_stats_add_far(f, E::up(x[tail]), kLog2e);
     return row_stats_lanes<64>(f, kLog2e);
   });
   if (lane == 0) {
@@ -310,7 +386,9 @@ struct ScoreGradArgs {
 };
 
 // d log p_t / d x_j = [j = t] - p_j,   d H / d x_j = -p_j (log p_j + H)
-// Element by element, so a row is cut into shares of kGradPieces pieces a thread.
+// Element by element, so a row is cut into shares of kGradPieces pieces a thread.  Bound by one read
+// and one write: 10240 rows of 10000 in fp32 124 us (5.8 TB/s of both, a quarter padding that is not read), 1271 of
+// 50001 in fp16 44 us (5.5 TB/s).
 constexpr int kGradPieces = 4;
 
 template <int DTYPE, bool STREAM>
@@ -333,7 +411,7 @@ __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs 
     const float zero[E::kVec] = {};
 #pragma unroll
     for (int j = 0; j < kGradPieces; ++j)
-      if (first + j * NT < pieces) 
+      if (first + j * NT < pieces)
         Piece<DTYPE, E::kVec>::template store<STREAM>(g + (size_t)(first + j * NT) * E::kVec, zero);
     if (has_tail) g[tail] = E::down(0.f);
     return;
@@ -403,9 +481,12 @@ __device__ __forceinline__ void lds_barrier() {
 // p = soft-max of the row at tau;   d loss / d x_j = tau (p_j - sum over k with id_k = j of q_k)
 //
 // A workgroup reads a row into registers, sums it, and writes the gradient from there; one barrier
-// hands the waves' sums and the teacher's q round.  (A workgroup that goes through several rows and reads the next one into a
-// second set of registers was slower, 158 against 122 us for 2560 rows of 50000 in bf16: the
-// registers cost it half of its neighbours, which hide the same latency.)
+// hands the waves' sums and the teacher's q round.  Bound by one read and one write: 10240 rows of
+// 10000 in fp32 135 us with a quarter padding.  2048 of 50000 in bf16 take 97 us (4.0 TB/s): three
+// such rows fit a compute unit, and reading, summing and writing overlap only between them.  (A
+// workgroup that goes through several rows and reads the next one into a second set of registers was
+// slower, 158 against 122 us for 2560 rows: the registers cost it half of its neighbours, which
+// hide the same latency.)
 //
 // The second launch bound holds a thread to the registers that 8 waves a SIMD leave (7 and 6 for 10 and
 // 13 pieces); without it 4000 rows of 20000 in fp32 take 161 instead of 120 us.

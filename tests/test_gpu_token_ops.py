@@ -194,6 +194,41 @@ def test_alternatives_among_ties_and_in_any_order(kind, V):
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("V", [7, 100, 2049, 40003, 270001])
+def test_alternatives_of_rows_with_few_columns_left(kind, V):
+    """Vocabularies masked but for some columns, to -inf, to the type's lowest value or to NaN: the
+    columns left over follow those in order, also where whole shares of a row have none."""
+    rng = np.random.default_rng(V + 1)
+    rows = []
+    for left in (0, 1, 5, 31, 32, 40, 129, 700, 5000):
+        for gone in (-np.inf, LOWEST[kind]):
+            for level in (0.0, 1.0):              # the same value everywhere, or spread
+                r = np.full(V, gone)
+                at = rng.permutation(V)[:left]
+                r[at] = 2.0 + level * rng.standard_normal(len(at))
+                rows.append(r)
+    for lo, hi in ((0, V // 9), (V // 2, V), (V - 3, V), (V // 3, V // 3 + 2)):
+        r = np.full(V, -np.inf)
+        r[lo:hi] = rng.standard_normal(hi - lo)
+        rows.append(r)
+        rows.append(np.where(np.isinf(r), LOWEST[kind], r))
+    r = np.full(V, -np.inf)                       # lowest values and -inf, nothing else
+    r[::3] = LOWEST[kind]
+    rows.append(r)
+    r = rng.standard_normal(V)                    # the better half stands behind, its values alike
+    r[V // 2:] = 9.0
+    rows.append(r)
+    r = np.where(rng.random(V) < 0.5, 0.0, -0.0)
+    rows.append(r)
+    x = np.stack(rows).astype(np.float32)
+    tokens = rng.integers(0, V, len(rows))
+    for k in (1, min(V, 6), min(V, 32)):
+        _check_score(_dev(x, kind), tokens, k=k, what="V=%d k=%d" % (V, k))
+        _check_score(_dev(x[-1:], kind), tokens[-1:], k=k)
+    _check_score(_dev(np.concatenate([x] * 20)[:, :min(V, 2049)], kind), np.tile(tokens % min(V, 2049), 20), k=min(V, 7))
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
 def test_rows_apart_from_each_other(kind):
     """Leading dimensions, the first positions of a [B,T,V] tensor, transposed and broadcast rows."""
     rng = np.random.default_rng(5)
