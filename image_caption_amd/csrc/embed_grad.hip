@@ -11,7 +11,8 @@ namespace {
 // second time and writes the same values to them.
 __device__ __forceinline__ int piece_col(int c, int n, int D) { return min(c, D - n); }
 
-// One group of lanes per token, kLookupAhead tokens at a time.
+// One group of lanes per token, kLookupAhead tokens at a time.  Bound by the writes: 131072 rows of 512
+// in bf16 take 28 us (4.8 TB/s written; the table stays in the caches).
 constexpr int kLookupAhead = 4;
 
 template <int DTYPE, int n, bool STREAM>
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_split_kernel(SortArgs p
 // the counts, so nothing depends on timing, and no workgroup waits for another.
 // SPLIT: its tokens come from the lists of embed_split_kernel.  Otherwise it reads all of them, 256 x N
 // in all from the caches, which for few tokens is less than a launch: 10240 take 8 us, 131071 took
-// 34 us and take 12 by way of the lists.
+// 34 us and take 18 by way of the lists, 6 of them the lists.
 template <bool SPLIT>
 __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(SortArgs p) {
   __shared__ int s_cnt[kSortWaves][kSortRows];
@@ -312,7 +313,8 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(SortArgs p)
 // `part` for each chunk it reaches (slot 0: the row of the chunk's first token, slot 1: the row of
 // its last one, if another); the chunk where it starts puts it on the list of long rows, and
 // embed_join_kernel adds its shares up in the chunks' order.  Rows without tokens get their zeros
-// from further waves, kZeroSlots of them each.
+// from further waves, kZeroSlots of them each.  131071 rows of 512 in bf16 into 50000 take 39 us (4.5
+// TB/s): rows of 1 kB in the order of the words, and the latency of where a chunk begins.
 struct SumArgs {
   const void* grad;
   void* dtable;
@@ -415,7 +417,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(SumArgs p) {
 constexpr int kJoinWaves = 4;
 
 // The long rows, one workgroup each in turn; its waves take the shares in turn, 64 columns at a
-// time.  The order of the list depends on timing, the sum of a row does not.
+// time.  The order of the list depends on timing, the sum of a row does not.  6 us for 131071 tokens,
+// most of it a launch and one pass of the most frequent word's shares.
 template <int DTYPE>
 __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(SumArgs p) {
   typedef Elem<DTYPE> E;

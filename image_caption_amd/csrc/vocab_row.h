@@ -244,18 +244,6 @@ __device__ __forceinline__ RowStats row_stats_lanes(RowStats a, float rate) {
   return a;
 }
 
-// Over a workgroup of WAVES waves; every thread gets the result.  s_part: WAVES entries of LDS.
-template <int WAVES>
-__device__ __forceinline__ RowStats row_stats_block(RowStats a, float rate, RowStats* s_part) {
-  a = row_stats_lanes<64>(a, rate);
-  if constexpr (WAVES > 1) {
-    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = row_stats_lanes<WAVES>(s_part[threadIdx.x & (WAVES - 1)], rate);
-  }
-  return a;
-}
-
 // One element of a row whose maximum m is known and so large that rate * x would overflow or round off
 // what tells the elements apart: y = rate (x - m).
 __device__ __forceinline__ void row_stats_add_far(RowStats& a, float x, float rate) {
@@ -387,16 +375,6 @@ struct Row {
       row_sum_add(a.s, v, rate, c);
     }
     return a;
-  }
-
-  // The row's statistics, the same in every thread (entropy: not among them)
-  __device__ __forceinline__ RowResult result(float rate, RowStats* s_part) const {
-    return row_result(row_stats_block<WAVES>(sums(rate), rate, s_part), rate, [&](float m) {
-      RowStats f = {m, 0.f, 0.f};
-      for (int i = threadIdx.x; i < V; i += kThreads) row_stats_add_far(f, E::up(x[i]), rate);
-      if constexpr (WAVES > 1) __syncthreads();
-      return row_stats_block<WAVES>(f, rate, s_part);
-    });
   }
 
   // out[column] = factor * exp((value - m) / tau - log_s) in the row's type; out may be the row
