@@ -187,7 +187,7 @@ __device__ __forceinline__ RowStats row_stats_empty() { return {kLowest, 0.f, 0.
 
 // Held within +-2^24, where the rounding of rate * m is at most one: a part further below has
 // y <= 0 and next to no weight beside any other, and a row whose own maximum is further out is summed
-// another way (Row::stats_far).
+// another way (row_stats_add_far).
 constexpr float kRefLimit = 16777216.f;
 __device__ __forceinline__ float row_ref(float m, float rate) {
   return fminf(fmaxf(m * rate, -kRefLimit), kRefLimit);

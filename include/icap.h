@@ -579,7 +579,8 @@ int icap_sample_categorical_f32(const float* logits, const float* u, const int32
  *   (r / rows_inner) * ld_outer + (r % rows_inner) * ld
  * of `logits` (rows_inner >= N: a matrix of leading dimension ld; rows_inner = T - 1: the first
  * T - 1 positions of a [B,T,V] tensor), at any element alignment.  A logit of -inf takes no part;
- * a row of nothing else has no distribution.  NaN or +inf in a row makes its floating results NaN. */
+ * a row of nothing else has no distribution.  NaN or +inf in a row makes its floating results NaN
+ * (the maximum in stats passes a NaN over). */
 
 /* Log probabilities of given tokens with the entropy of their rows and the best alternatives.
  *   p_j = exp(x_j) / sum_i exp(x_i);  log_probs[n] = log p_tokens[n];

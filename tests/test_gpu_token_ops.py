@@ -229,6 +229,28 @@ def test_alternatives_of_rows_with_few_columns_left(kind, V):
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("V", [3, 500, 30011])
+def test_rows_of_nan(kind, V):
+    """Rows of NaN alone, or of NaN and -inf: no number comes out of them, and nothing but them."""
+    from image_caption_amd import ops
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((4, V)).astype(np.float32)
+    x[1] = np.nan
+    x[2] = -np.inf
+    x[2, V // 2] = np.nan
+    tokens, k = rng.integers(0, V, 4), min(V, 6)
+    xd = _dev(x, kind)
+    lp, h, stats, ids, top = ops.token_log_probs(xd, _ids(tokens), top_k=k)
+    g = ops.token_log_probs_grad(xd, _ids(tokens), stats, h, torch.ones_like(lp), torch.ones_like(h))
+    loss, dg = ops.distill_loss(xd, torch.zeros(4, 2, device=dev()), _ids(rng.integers(0, V, (4, 2))), 1.5,
+                                torch.ones_like(lp))
+    for got in (lp, h, stats[:, 1], top, g, loss, dg):
+        nan = torch.isnan(got).reshape(4, -1)
+        assert nan[1:3].all() and not nan[[0, 3]].any()
+    np.testing.assert_array_equal(np_of(ids)[1:3], [list(range(k))] * 2)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
 def test_rows_apart_from_each_other(kind):
     """Leading dimensions, the first positions of a [B,T,V] tensor, transposed and broadcast rows."""
     rng = np.random.default_rng(5)
