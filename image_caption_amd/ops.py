@@ -500,6 +500,8 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
             teacher_logits.shape != teacher_ids.shape:
         raise ValueError("distill_loss: teacher_logits and teacher_ids must be [..., K] for logits [..., V]")
     shape, V, K = logits.shape[:-1], logits.shape[-1], teacher_ids.shape[-1]
+    if V == 0:
+        raise ValueError("distill_loss: logits have no columns")
     if not 1 <= K <= _lib.MAX_TEACHER_LOGITS:
         raise ValueError("distill_loss: the teacher must hand over 1 .. %d logits" % _lib.MAX_TEACHER_LOGITS)
     if grad_loss is not None and grad_loss.shape != shape:
@@ -514,7 +516,7 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
     if grad_loss is not None:
         out = _grad_out(out, logits, "distill_loss")
         g = _chk(out, DTYPES, "out", rows=True)
-    if N and V:
+    if N:
         inner, ld, ld_outer, out_ld, out_ld_outer = _row_strides(logits, logits if out is None else out)
         _call("icap_distill_loss", x, DTYPES[logits.dtype], N, V, inner, ld, ld_outer, tx,
               DTYPES[teacher_logits.dtype], ti, K, float(temperature), gl, loss.data_ptr(), g, out_ld,
