@@ -537,7 +537,7 @@ __global__ __launch_bounds__(WAVES * 64, NV == 13 ? 6 : NV == 10 ? 7 : 8) void d
       float t = -INFINITY, xk = 0.f;
       if (id != -1) t = bits_value(k < 64 ? t0 : load_bits(p.t_logits, p.t_dtype, (size_t)row * p.K + k), p.t_dtype);
       if (in) xk = bits_value(k < 64 ? x0 : load_bits(x, DTYPE, id), DTYPE);
-      bad |= id != -1 && !in;
+      bad |= id != -1 && !in && !(t == -INFINITY);      // (an absent entry's id says nothing)
       entries |= !(t == -INFINITY);
       top = fmaxf(top, t);
       s_id[k] = in ? id : -1;

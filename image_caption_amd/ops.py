@@ -495,7 +495,8 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
     loss = temperature^2 * KL(softmax(teacher_logits / temperature) over the K entries ||
     softmax(logits / temperature)).  With grad_loss [...] also the gradient of
     sum(grad_loss * loss) to the logits, [..., V] in their dtype, in the same call (out=logits
-    overwrites them).  An entry with id -1 is absent; a row without entries gives zeros."""
+    overwrites them).  An entry with id -1, or with a logit of -inf whatever its id, is absent; a row
+    without entries gives zeros; any other id outside 0 .. V - 1 makes its row NaN."""
     if logits.dim() == 0 or teacher_ids.dim() == 0 or teacher_ids.shape[:-1] != logits.shape[:-1] or \
             teacher_logits.shape != teacher_ids.shape:
         raise ValueError("distill_loss: teacher_logits and teacher_ids must be [..., K] for logits [..., V]")
