@@ -418,11 +418,12 @@ __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs 
   }
   if ((token < 0 || token >= p.V) && g_lp != 0.f) g_lp = NAN;
   const float inv_s = __builtin_amdgcn_exp2f(-log_s * kLog2e);
+  // (e u before g_h: where e is 0 - a masked logit - g_h u may pass fp32's range, and 0 inf is NaN)
   auto grad = [&](float v, int c) {
     const float d = v - m;
     const float e = __builtin_amdgcn_exp2f(d * kLog2e) * inv_s;
     const float u = fmaxf(d, kFarBelow) - log_s + h;
-    return -e * (g_lp + g_h * u) + (c == token ? g_lp : 0.f);
+    return (c == token ? g_lp : 0.f) - __builtin_fmaf(g_h, e * u, e * g_lp);
   };
   u32x4 raw[kGradPieces];
   float t = 0.f;

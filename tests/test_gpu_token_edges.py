@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_token_ops import TYPES, _check_distill_rows, _dev, _ids, _logits
+from tests.helpers import dev
+from tests.test_gpu_token_ops import LOWEST, TYPES, _check_distill_rows, _dev, _ids, _logits
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +37,29 @@ def test_teacher_entry_at_minus_inf_is_absent_whatever_its_id(kind, V):
         assert loss[6] == 0 and not grad[6].any()
         assert loss[7:].isnan().all() and grad[7:].isnan().all()
         _check_distill_rows(x, t, named, 2.0, g, kind, ())
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("V", [9, 3000])
+@pytest.mark.parametrize("size", [1.0, 1e9, 1e20, 1e36])
+def test_gradient_of_masked_columns_is_zero_however_large_the_entropy_weight(kind, V, size):
+    """p log p is 0 where p is.  Elsewhere a weight past fp16's range may give infinities, never a NaN."""
+    from image_caption_amd import ops
+    rng = np.random.default_rng(V)
+    N = 4
+    x = rng.standard_normal((N, V)).astype(np.float32)
+    masked = np.zeros((N, V), bool)
+    masked[:, ::3] = True
+    masked[3] = True
+    masked[3, 1] = False                     # one column is left: its gradient is 0 as well
+    x[masked] = -np.inf
+    x[1, masked[1]] = LOWEST[kind]
+    x = _dev(x, kind)
+    tokens = _ids(np.ones(N))
+    _, h, stats, _, _ = ops.token_log_probs(x, tokens)
+    g_h = _dev(np.full(N, size))
+    for g_lp in (None, _dev(np.ones(N))):
+        for sign in (1, -1):
+            got = ops.token_log_probs_grad(x, tokens, stats, h, g_lp, sign * g_h)
+            assert not got[torch.as_tensor(masked, device=dev())].any()
+            assert not got.isnan().any()
