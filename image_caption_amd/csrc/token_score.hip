@@ -407,7 +407,8 @@ __global__ __launch_bounds__(NT) void token_log_probs_grad_kernel(ScoreGradArgs 
   const int pieces = p.V / E::kVec, first = share * NT * kGradPieces + tid;
   const int tail = pieces * E::kVec + tid;
   const bool has_tail = share == p.shares - 1 && tail < p.V;
-  if (token == p.pad || m == -INFINITY || (g_lp == 0.f && g_h == 0.f)) {
+  const bool none = m == -INFINITY && log_s == log_s;      // (a row of NaN and -inf has that maximum too)
+  if (token == p.pad || none || (g_lp == 0.f && g_h == 0.f)) {
     const float zero[E::kVec] = {};
 #pragma unroll
     for (int j = 0; j < kGradPieces; ++j)

@@ -175,15 +175,14 @@ __device__ __forceinline__ void store_vec(typename Elem<DTYPE>::type* x, int col
 //   y = rate * x - c (one fused multiply-add),   s = sum 2^y,   w = sum 2^y y.
 // c is rate * m rounded; it is the same number for every element, so its rounding cancels.
 //   log2 of the sum = c + log2 s,   entropy = ln 2 (log2 s - w / s)
-// Parts join in a tree of a fixed shape, so a row's result does not depend on timing.  m starts at
-// the lowest float instead of -inf, so that a part of -inf alone has s = 0 and no NaN.  A NaN, and
-// the inf - inf of an infinite maximum, end in s and stay.
+// Parts join in a tree of a fixed shape, so a row's result does not depend on timing.  A part of -inf
+// alone has m = -inf and, as its reference is finite (row_ref), s = 0 and no NaN.  A NaN, and the
+// inf - inf of an infinite maximum, end in s and stay; m passes a NaN over.
 struct RowStats {
   float m, s, w;
 };
-constexpr float kLowest = -3.4028234663852886e38f;
 
-__device__ __forceinline__ RowStats row_stats_empty() { return {kLowest, 0.f, 0.f}; }
+__device__ __forceinline__ RowStats row_stats_empty() { return {-INFINITY, 0.f, 0.f}; }
 
 // Held within +-2^24, where the rounding of rate * m is at most one: a part further below has
 // y <= 0 and next to no weight beside any other, and a row whose own maximum is further out is summed
@@ -255,7 +254,7 @@ __device__ __forceinline__ void row_stats_add_far(RowStats& a, float x, float ra
 
 // What a row's joined statistics say; far(m) sums the row again by row_stats_add_far.
 struct RowResult {
-  float m;          // the maximum
+  float m;          // the maximum; -inf in a row without a number: all -inf, or NaN as well
   float log_s;      // ln sum exp((x - m) / tau)
   float entropy;
   bool none;        // every element is -inf
@@ -267,7 +266,7 @@ __device__ __forceinline__ RowResult row_result(RowStats a, float rate, Far far)
   const float c = row_ref(a.m, rate);
   float off = __builtin_fmaf(a.m, rate, -c);      // of the maximum from the reference
   RowResult r;
-  r.far = !(fabsf(c) < kRefLimit);
+  r.far = !(fabsf(c) < kRefLimit) && a.m != -INFINITY;
   if (r.far) {
     a = far(a.m);
     off = 0.f;
@@ -276,7 +275,7 @@ __device__ __forceinline__ RowResult row_result(RowStats a, float rate, Far far)
   r.s = a.s;
   const float log_s = logf(a.s);
   r.none = a.s == 0.f;
-  r.m = r.none ? -INFINITY : a.m;
+  r.m = a.m;
   r.log_s = r.none ? 0.f : log_s - off * kLn2;
   r.entropy = r.none ? 0.f : log_s - kLn2 * (a.w / a.s);
   return r;

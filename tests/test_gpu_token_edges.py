@@ -3,8 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.helpers import dev
-from tests.test_gpu_token_ops import LOWEST, TYPES, _check_distill_rows, _dev, _ids, _logits
+from tests.helpers import dev, np_of
+from tests.test_gpu_token_ops import LOWEST, TYPES, _check_distill_rows, _dev, _f64, _ids, _logits
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,36 @@ def test_gradient_of_masked_columns_is_zero_however_large_the_entropy_weight(kin
             got = ops.token_log_probs_grad(x, tokens, stats, h, g_lp, sign * g_h)
             assert not got[torch.as_tensor(masked, device=dev())].any()
             assert not got.isnan().any()
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("V", [2, 3, 500, 3001, 30011, 140001])
+@pytest.mark.parametrize("N", [5, 700])
+def test_the_maximum_passes_a_nan_over(kind, V, N):
+    """Rows of NaN beside -inf, beside the lowest value, beside numbers, and alone."""
+    from image_caption_amd import ops
+    if N * V > 1 << 24:
+        N = 60
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((N, V)).astype(np.float32)
+    x[0], x[1], x[2], x[3] = -np.inf, np.nan, LOWEST[kind], -np.inf
+    x[0, V - 1] = x[2, 0] = x[4, V // 2] = np.nan
+    want = np.where(np.isnan(x), -np.inf, _f64(_dev(x, kind))).max(1)
+    x = _dev(x, kind)
+    for top_k in (0, 2):
+        lp, h, stats, ids, top = ops.token_log_probs(x, _ids(np.zeros(N)), top_k=top_k)
+        np.testing.assert_array_equal(_f64(stats[:, 0]), want)
+        nan = [0, 1, 2, 4]
+        assert stats[nan, 1].isnan().all() and lp[nan].isnan().all() and h[nan].isnan().all()
+        assert torch.equal(stats[3], stats.new_tensor([float("-inf"), 0])) and lp[3] == float("-inf") and h[3] == 0
+        if top_k:
+            np.testing.assert_array_equal(np_of(ids)[[0, 1, 3]], [[0, 1]] * 3)
+            assert top[nan].isnan().all() and (top[3] == float("-inf")).all()
+    ones = _dev(np.ones(N))
+    got = ops.token_log_probs_grad(x, _ids(np.zeros(N)), stats, h, ones, ones)
+    assert got[nan].isnan().all() and not got[3].any()
+    assert torch.isfinite(got[5:].float()).all()
+    loss, got = ops.distill_loss(x, _dev(np.zeros((N, 2))), _ids(np.zeros((N, 2))), 1.5, ones)
+    assert loss[nan].isnan().all() and got[nan].isnan().all()
+    assert loss[3] == float("inf") and not got[3].any()
+    assert torch.isfinite(loss[5:]).all() and torch.isfinite(got[5:].float()).all()
