@@ -396,6 +396,14 @@ def sample_categorical(logits, u, step=0, row_len=None, start_token=-1, eos_toke
 # Forward and gradient are calls of their own, as everywhere in this module (torch supplies memory
 # and streams, not the graph of a backward pass).
 
+def _int32(value, name):
+    """A number the library takes as a 32-bit integer, to which ctypes would cut it without a word."""
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError("%s %d does not fit 32 bits" % (name, value))
+    return value
+
+
 def _row_split(t, name):
     """(rows_inner, ld, ld_outer) of a tensor [..., V] with contiguous rows: see icap.h."""
     V = t.shape[-1]
@@ -447,7 +455,8 @@ def token_log_probs(logits, tokens, top_k=0, pad_token=-1):
     equal logits by the lower id.  Rows whose token is pad_token are left out: zeros, ids of -1."""
     if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
         raise ValueError("token_log_probs: logits must be [..., V] for tokens [...]")
-    V, N, dev, shape, top_k = logits.shape[-1], tokens.numel(), logits.device, tokens.shape, int(top_k)
+    dev, shape, top_k, pad_token = logits.device, tokens.shape, int(top_k), _int32(pad_token, "pad_token")
+    V, N = _int32(logits.shape[-1], "vocabulary"), _int32(tokens.numel(), "number of rows")
     if not 0 <= top_k <= min(V, _lib.MAX_ALTERNATIVES):
         raise ValueError("token_log_probs: top_k must be in 0 .. min(V, %d)" % _lib.MAX_ALTERNATIVES)
     x, t = _chk(logits, DTYPES, "logits", rows=True), _chk(tokens, i32, "tokens")
@@ -458,7 +467,7 @@ def token_log_probs(logits, tokens, top_k=0, pad_token=-1):
     top_lp = torch.empty_like(top_ids, dtype=f32) if top_k else None
     if N:
         _call("icap_token_log_probs", x, DTYPES[logits.dtype], N, V, *_row_split(logits, "logits"), t,
-              int(pad_token), top_k, log_probs.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+              pad_token, top_k, log_probs.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
               top_ids.data_ptr() if top_k else None, top_lp.data_ptr() if top_k else None,
               current_stream())
     return log_probs, entropy, stats, top_ids, top_lp
@@ -476,7 +485,8 @@ def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, gr
     for g in (grad_log_probs, grad_entropy):
         if g is not None and g.shape != tokens.shape:
             raise ValueError("token_log_probs_grad: gradients must have the tokens' shape")
-    V, N = logits.shape[-1], tokens.numel()
+    V, N = _int32(logits.shape[-1], "vocabulary"), _int32(tokens.numel(), "number of rows")
+    pad_token = _int32(pad_token, "pad_token")
     out = _grad_out(out, logits, "token_log_probs_grad")
     args = (_chk(logits, DTYPES, "logits", rows=True), _chk(out, DTYPES, "out", rows=True),
             _chk(tokens, i32, "tokens"), _chk(stats, f32, "stats"), _chk(entropy, f32, "entropy"),
@@ -484,7 +494,7 @@ def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, gr
     if N and V:
         inner, ld, ld_outer, out_ld, out_ld_outer = _row_strides(logits, out)
         _call("icap_token_log_probs_grad", args[0], DTYPES[logits.dtype], N, V, inner, ld, ld_outer, args[2],
-              int(pad_token), *args[3:], args[1], out_ld, out_ld_outer, current_stream())
+              pad_token, *args[3:], args[1], out_ld, out_ld_outer, current_stream())
     return out
 
 
@@ -500,7 +510,8 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
     if logits.dim() == 0 or teacher_ids.dim() == 0 or teacher_ids.shape[:-1] != logits.shape[:-1] or \
             teacher_logits.shape != teacher_ids.shape:
         raise ValueError("distill_loss: teacher_logits and teacher_ids must be [..., K] for logits [..., V]")
-    shape, V, K = logits.shape[:-1], logits.shape[-1], teacher_ids.shape[-1]
+    shape, K = logits.shape[:-1], teacher_ids.shape[-1]
+    V, N = _int32(logits.shape[-1], "vocabulary"), _int32(shape.numel(), "number of rows")
     if V == 0:
         raise ValueError("distill_loss: logits have no columns")
     if not 1 <= K <= _lib.MAX_TEACHER_LOGITS:
@@ -510,7 +521,6 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
     if grad_loss is None and out is not None:
         raise ValueError("distill_loss: out needs grad_loss")
     loss = torch.empty(shape, dtype=f32, device=logits.device)
-    N = loss.numel()
     x, tx = _chk(logits, DTYPES, "logits", rows=True), _chk(teacher_logits, DTYPES, "teacher_logits")
     ti, gl = _chk(teacher_ids, i32, "teacher_ids"), _opt(grad_loss, f32, "grad_loss")
     g = None
@@ -528,12 +538,13 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
 def embedding_scaled(table, ids, scale=1.0, pad_token=-1):
     """scale * table[ids]: table [V,D] (float32, bfloat16 or float16), ids [...] int32 -> [..., D] in
     the table's dtype; zero rows for pad_token and for ids outside the table."""
-    V, D = table.shape
+    V, D = (_int32(n, "size of the table") for n in table.shape)
+    N, pad_token = _int32(ids.numel(), "number of rows"), _int32(pad_token, "pad_token")
     out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
     tab, i = _chk(table, DTYPES, "table"), _chk(ids, i32, "ids")
     if out.numel():
-        _call("icap_embedding_scaled", tab, DTYPES[table.dtype], i, out.data_ptr(), ids.numel(), V, D,
-              float(scale), int(pad_token), current_stream())
+        _call("icap_embedding_scaled", tab, DTYPES[table.dtype], i, out.data_ptr(), N, V, D,
+              float(scale), pad_token, current_stream())
     return out
 
 
@@ -542,7 +553,8 @@ def embedding_grad(grad, ids, vocab_size, scale=1.0, pad_token=-1):
     dtype.  Sums run in float32 in an order the ids alone decide: the same inputs, the same bits."""
     if grad.dim() == 0 or grad.shape[:-1] != ids.shape:
         raise ValueError("embedding_grad: grad must be [..., D] for ids [...]")
-    V, D, N, dev = int(vocab_size), grad.shape[-1], ids.numel(), grad.device
+    V, D, dev = _int32(vocab_size, "vocab_size"), _int32(grad.shape[-1], "size of a row"), grad.device
+    N, pad_token = _int32(ids.numel(), "number of rows"), _int32(pad_token, "pad_token")
     if V < 1:
         raise ValueError("embedding_grad: vocab_size must be positive")
     out = torch.empty(V, D, dtype=grad.dtype, device=dev)
@@ -553,7 +565,7 @@ def embedding_grad(grad, ids, vocab_size, scale=1.0, pad_token=-1):
         need = int(_lib.load().icap_embedding_grad_workspace_bytes(N, V, D))
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _call("icap_embedding_grad", g, DTYPES[grad.dtype], i, out.data_ptr(), N, V, D, float(scale),
-              int(pad_token), ws.data_ptr(), need, current_stream())
+              pad_token, ws.data_ptr(), need, current_stream())
     return out
 
 
