@@ -40,7 +40,7 @@ def test_numbers_past_32_bits():
     with pytest.raises(ValueError, match="rows"):
         ops.token_log_probs_grad(big, ids, st, h, out=big)
     with pytest.raises(ValueError, match="rows"):
-        ops.distill_loss(big, st, st.to(torch.int32)[:1].expand(many, 2))
+        ops.distill_loss(big, st, st[:1].to(torch.int32).expand(many, 2))
     with pytest.raises(ValueError, match="rows"):
         ops.embedding_scaled(x, ids)
     with pytest.raises(ValueError, match="rows"):
