@@ -445,6 +445,13 @@ def _row_strides(t, out):
     return (*split, *out_split[1:])
 
 
+def _overwritten(out, given):
+    """Tells torch that a caller's tensor has new contents, so that a graph that saved it does not go on
+    with them."""
+    if given:
+        torch.autograd.graph.increment_version(out)
+
+
 def token_log_probs(logits, tokens, top_k=0, pad_token=-1):
     """Log probabilities of `tokens` [...] int32 under the softmax of `logits` [..., V] (float32,
     bfloat16 or float16) -> (log_probs [...], entropy [...], stats [..., 2], top_ids [..., top_k],
@@ -487,7 +494,7 @@ def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, gr
             raise ValueError("token_log_probs_grad: gradients must have the tokens' shape")
     V, N = _int32(logits.shape[-1], "vocabulary"), _int32(tokens.numel(), "number of rows")
     pad_token = _int32(pad_token, "pad_token")
-    out = _grad_out(out, logits, "token_log_probs_grad")
+    given, out = out is not None, _grad_out(out, logits, "token_log_probs_grad")
     args = (_chk(logits, DTYPES, "logits", rows=True), _chk(out, DTYPES, "out", rows=True),
             _chk(tokens, i32, "tokens"), _chk(stats, f32, "stats"), _chk(entropy, f32, "entropy"),
             _opt(grad_log_probs, f32, "grad_log_probs"), _opt(grad_entropy, f32, "grad_entropy"))
@@ -495,6 +502,7 @@ def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, gr
         inner, ld, ld_outer, out_ld, out_ld_outer = _row_strides(logits, out)
         _call("icap_token_log_probs_grad", args[0], DTYPES[logits.dtype], N, V, inner, ld, ld_outer, args[2],
               pad_token, *args[3:], args[1], out_ld, out_ld_outer, current_stream())
+        _overwritten(out, given)
     return out
 
 
@@ -523,7 +531,7 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
     loss = torch.empty(shape, dtype=f32, device=logits.device)
     x, tx = _chk(logits, DTYPES, "logits", rows=True), _chk(teacher_logits, DTYPES, "teacher_logits")
     ti, gl = _chk(teacher_ids, i32, "teacher_ids"), _opt(grad_loss, f32, "grad_loss")
-    g = None
+    g, given = None, out is not None
     if grad_loss is not None:
         out = _grad_out(out, logits, "distill_loss")
         g = _chk(out, DTYPES, "out", rows=True)
@@ -532,6 +540,7 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
         _call("icap_distill_loss", x, DTYPES[logits.dtype], N, V, inner, ld, ld_outer, tx,
               DTYPES[teacher_logits.dtype], ti, K, float(temperature), gl, loss.data_ptr(), g, out_ld,
               out_ld_outer, current_stream())
+        _overwritten(out, given)
     return loss, out
 
 

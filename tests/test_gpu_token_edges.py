@@ -96,3 +96,27 @@ def test_the_maximum_passes_a_nan_over(kind, V, N):
     assert loss[nan].isnan().all() and got[nan].isnan().all()
     assert loss[3] == float("inf") and not got[3].any()
     assert torch.isfinite(loss[5:]).all() and torch.isfinite(got[5:].float()).all()
+
+
+@pytest.mark.parametrize("inside", [False, True])
+def test_overwritten_logits_are_noticed_by_a_backward_pass(inside):
+    """A graph that saved the logits must not go on with the gradient that took their place."""
+    from image_caption_amd import ops
+    N, V = 5, 60
+    tokens, g = _ids(np.arange(N)), _dev(np.ones(N))
+    for op in ("scores", "distillation"):
+        w = torch.randn(N, V, device=dev(), requires_grad=True)
+        x = w.exp()                              # whose backward pass reads x
+        flat = x.detach()
+        out = flat if inside else torch.empty_like(flat)
+        if op == "scores":
+            _, h, stats, _, _ = ops.token_log_probs(flat, tokens)
+            ops.token_log_probs_grad(flat, tokens, stats, h, g, g, out=out)
+        else:
+            ops.distill_loss(flat, _dev(np.zeros((N, 2))), _ids(np.zeros((N, 2))), 1.0, g, out=out)
+        if inside:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                x.sum().backward()
+        else:
+            x.sum().backward()
+            assert torch.equal(w.grad, x.detach())
