@@ -5,6 +5,7 @@ tensors (ROCm device, dtype, contiguity, shape) and hands raw device pointers pl
 the current HIP stream to the C ABI."""
 from __future__ import annotations
 
+import math
 import sys
 import threading
 
@@ -422,6 +423,19 @@ def _extent(t):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _apart(a, b):
+    """Whether two tensors of contiguous rows share no byte.  Where their extents meet: every row of
+    either begins a multiple of `step` behind its first, so one's rows may lie between the other's."""
+    if not a.numel() or not b.numel() or a.device != b.device:
+        return True
+    (a0, a_end), (b0, b_end) = _extent(a), _extent(b)
+    if a_end <= b0 or b_end <= a0:
+        return True
+    width_a, width_b = ((t.shape[-1] if t.dim() else 1) * t.element_size() for t in (a, b))
+    step = math.gcd(*(st * t.element_size() for t in (a, b) for n, st in zip(t.shape[:-1], t.stride()) if n > 1))
+    return step > 0 and width_b <= (a0 - b0) % step <= step - width_a
+
+
 def _grad_out(out, like, name):
     """The gradient's tensor: a new one, or the caller's if it fits - the logits themselves, or
     memory apart from them."""
@@ -429,10 +443,9 @@ def _grad_out(out, like, name):
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError("%s: out must have the logits' shape and dtype" % name)
-    if out.numel() and not (out.data_ptr() == like.data_ptr() and out.stride() == like.stride()):
-        (a, a_end), (b, b_end) = _extent(out), _extent(like)
-        if out.device == like.device and a < b_end and b < a_end:
-            raise ValueError("%s: out overlaps the logits without being them" % name)
+    same = out.data_ptr() == like.data_ptr() and out.stride() == like.stride()
+    if not same and not _apart(out, like):
+        raise ValueError("%s: out overlaps the logits without being them" % name)
     return out
 
 

@@ -120,3 +120,25 @@ def test_overwritten_logits_are_noticed_by_a_backward_pass(inside):
         else:
             x.sum().backward()
             assert torch.equal(w.grad, x.detach())
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_gradient_between_the_rows_of_the_logits(kind):
+    """Logits and gradient side by side in the rows of one buffer."""
+    from image_caption_amd import ops
+    rng = np.random.default_rng(2)
+    N, V, K = 7, 301, 5
+    tokens, g = _ids(rng.integers(0, V, N)), _dev(rng.standard_normal(N))
+    ti, tl = _ids(rng.integers(0, V, (N, K))), _logits(rng, N, K, "f32")
+    for first, second in ((0, V), (V + 3, 2)):
+        buf = _logits(rng, N, 2 * V + 3, kind)
+        x, out = buf[:, first:first + V], buf[:, second:second + V]
+        _, h, stats, _, _ = ops.token_log_probs(x, tokens)
+        want = ops.token_log_probs_grad(x, tokens, stats, h, g, g)
+        loss, d_want = ops.distill_loss(x, tl, ti, 2.0, g)
+        keep = buf.clone()
+        keep[:, second:second + V] = want
+        assert ops.token_log_probs_grad(x, tokens, stats, h, g, g, out=out) is out and torch.equal(buf, keep)
+        keep[:, second:second + V] = d_want
+        again, d = ops.distill_loss(x, tl, ti, 2.0, g, out=out)
+        assert d is out and torch.equal(again, loss) and torch.equal(buf, keep)

@@ -45,3 +45,28 @@ def test_numbers_past_32_bits():
         ops.embedding_scaled(x, ids)
     with pytest.raises(ValueError, match="rows"):
         ops.embedding_grad(big, ids, 10)
+
+
+def test_gradient_between_the_rows_of_the_logits_and_over_them():
+    from image_caption_amd import ops
+    _, t, st, h = _inputs(6)
+    buf = torch.zeros(6, 20)
+    g = torch.zeros(6)
+    # between the rows of the logits: past the check, then refused for not being on the GPU
+    for x, out in ((buf[:, :8], buf[:, 8:16]), (buf[:, 12:], buf[:, 2:10]), (buf[:, :8], buf[:, 12:]),
+                   (buf[::2, :8], buf[1::2, 4:12])):
+        n = len(x)
+        with pytest.raises(ValueError, match="GPU"):
+            ops.token_log_probs_grad(x, t[:n], st[:n], h[:n], g[:n], out=out)
+    cube = buf.view(2, 3, 20)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.token_log_probs_grad(cube[:, :2, :8], t[:4].view(2, 2), st[:4].view(2, 2, 2), h[:4].view(2, 2),
+                                 g[:4].view(2, 2), out=cube[:, 1:, 8:16])
+    # over them
+    for x, out in ((buf[:, :8], buf[:, 7:15]), (buf[:, 12:], buf[:, 5:13]), (buf[:5, :8], buf[1:, :8]),
+                   (buf[:5, 12:], buf.as_strided((5, 8), (18, 1), 30)), (cube[:, :2, :8], cube[:, 1:, :8])):
+        shape = x.shape[:-1]
+        n = shape.numel()
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.token_log_probs_grad(x, t[:n].view(shape), st[:n].view(*shape, 2), h[:n].view(shape), g[:n].view(shape),
+                                     out=out)
