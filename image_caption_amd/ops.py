@@ -436,9 +436,9 @@ def _apart(a, b):
     return step > 0 and width_b <= (a0 - b0) % step <= step - width_a
 
 
-def _grad_out(out, like, name):
+def _grad_out(out, like, name, **others):
     """The gradient's tensor: a new one, or the caller's if it fits - the logits themselves, or
-    memory apart from them."""
+    memory apart from them, and apart from the other operands."""
     if out is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
     if out.shape != like.shape or out.dtype != like.dtype:
@@ -446,6 +446,9 @@ def _grad_out(out, like, name):
     same = out.data_ptr() == like.data_ptr() and out.stride() == like.stride()
     if not same and not _apart(out, like):
         raise ValueError("%s: out overlaps the logits without being them" % name)
+    for operand, t in others.items():
+        if t is not None and not _apart(out, t):
+            raise ValueError("%s: out overlaps %s" % (name, operand))
     return out
 
 
@@ -507,7 +510,9 @@ def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, gr
             raise ValueError("token_log_probs_grad: gradients must have the tokens' shape")
     V, N = _int32(logits.shape[-1], "vocabulary"), _int32(tokens.numel(), "number of rows")
     pad_token = _int32(pad_token, "pad_token")
-    given, out = out is not None, _grad_out(out, logits, "token_log_probs_grad")
+    given, out = out is not None, _grad_out(
+        out, logits, "token_log_probs_grad", tokens=tokens, stats=stats, entropy=entropy,
+        grad_log_probs=grad_log_probs, grad_entropy=grad_entropy)
     args = (_chk(logits, DTYPES, "logits", rows=True), _chk(out, DTYPES, "out", rows=True),
             _chk(tokens, i32, "tokens"), _chk(stats, f32, "stats"), _chk(entropy, f32, "entropy"),
             _opt(grad_log_probs, f32, "grad_log_probs"), _opt(grad_entropy, f32, "grad_entropy"))
@@ -541,13 +546,14 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
         raise ValueError("distill_loss: grad_loss must have one value per row of the logits")
     if grad_loss is None and out is not None:
         raise ValueError("distill_loss: out needs grad_loss")
+    given = out is not None
+    if grad_loss is not None:
+        out = _grad_out(out, logits, "distill_loss", teacher_logits=teacher_logits, teacher_ids=teacher_ids,
+                        grad_loss=grad_loss)
     loss = torch.empty(shape, dtype=f32, device=logits.device)
     x, tx = _chk(logits, DTYPES, "logits", rows=True), _chk(teacher_logits, DTYPES, "teacher_logits")
     ti, gl = _chk(teacher_ids, i32, "teacher_ids"), _opt(grad_loss, f32, "grad_loss")
-    g, given = None, out is not None
-    if grad_loss is not None:
-        out = _grad_out(out, logits, "distill_loss")
-        g = _chk(out, DTYPES, "out", rows=True)
+    g = None if out is None else _chk(out, DTYPES, "out", rows=True)
     if N:
         inner, ld, ld_outer, out_ld, out_ld_outer = _row_strides(logits, logits if out is None else out)
         _call("icap_distill_loss", x, DTYPES[logits.dtype], N, V, inner, ld, ld_outer, tx,

@@ -600,7 +600,7 @@ int icap_token_log_probs(const void* logits, int dtype, int N, int V, int rows_i
  * with stats and entropy as icap_token_log_probs wrote them; either gradient may be NULL (zero).
  * Rows of pad_token, without a distribution, or with both gradients zero are zeros and are not
  * read.  dlogits has the logits' dtype and row split, its own strides, and may be the logits
- * themselves (same strides). */
+ * themselves (same strides); otherwise it shares no element with any operand. */
 int icap_token_log_probs_grad(const void* logits, int dtype, int N, int V, int rows_inner, long long ld,
                               long long ld_outer, const int32_t* tokens, int pad_token,
                               const float* stats, const float* entropy, const float* grad_log_probs,

@@ -70,3 +70,25 @@ def test_gradient_between_the_rows_of_the_logits_and_over_them():
         with pytest.raises(ValueError, match="overlaps"):
             ops.token_log_probs_grad(x, t[:n].view(shape), st[:n].view(*shape, 2), h[:n].view(shape), g[:n].view(shape),
                                      out=out)
+
+
+def test_gradient_over_any_other_operand():
+    from image_caption_amd import ops
+    t, st, h, g = torch.zeros(4, dtype=torch.int32), torch.zeros(4, 2), torch.zeros(4), torch.zeros(4)
+    x, pool = torch.zeros(4, 8), torch.zeros(64)
+    out = pool[:32].view(4, 8)
+    for name, args in (("stats", (pool[24:32].view(4, 2), h, g, g)), ("entropy", (st, pool[31:35], g, g)),
+                       ("grad_log_probs", (st, h, pool[:4], g)), ("grad_entropy", (st, h, g, pool[8:12]))):
+        for o, y in ((out, x), (out, out)):
+            with pytest.raises(ValueError, match="overlaps " + name):
+                ops.token_log_probs_grad(y, t, *args, out=o)
+    with pytest.raises(ValueError, match="overlaps tokens"):
+        ops.token_log_probs_grad(x, pool.view(torch.int32)[4:8], st, h, g, g, out=out)
+    tl, ti = torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32)
+    for name, args in (("teacher_logits", (pool[8:16].view(4, 2), ti, 1.0, g)),
+                       ("teacher_ids", (tl, pool.view(torch.int32)[8:16].view(4, 2), 1.0, g)),
+                       ("grad_loss", (tl, ti, 1.0, pool[28:32]))):
+        with pytest.raises(ValueError, match="overlaps " + name):
+            ops.distill_loss(x, *args, out=out)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.distill_loss(x, tl, ti, 1.0, pool[32:36], out=out)
