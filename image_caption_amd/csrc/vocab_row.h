@@ -144,32 +144,6 @@ struct Piece<DTYPE, 1> {
   __device__ static __forceinline__ void store(type* p, const float (&x)[1]) { *p = Elem<DTYPE>::down(x[0]); }
 };
 
-// kVec elements from x + col; columns past the row's end read as `fill`.
-template <int DTYPE>
-__device__ __forceinline__ void load_vec(const typename Elem<DTYPE>::type* x, int col, int V,
-                                         float fill, float (&out)[Elem<DTYPE>::kVec]) {
-  constexpr int kVec = Elem<DTYPE>::kVec;
-  if (col + kVec <= V) {
-    Elem<DTYPE>::unpack(*reinterpret_cast<const u32x4_any*>(x + col), out);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) out[i] = col + i < V ? Elem<DTYPE>::up(x[col + i]) : fill;
-  }
-}
-
-template <int DTYPE>
-__device__ __forceinline__ void store_vec(typename Elem<DTYPE>::type* x, int col, int V,
-                                          const float (&v)[Elem<DTYPE>::kVec]) {
-  constexpr int kVec = Elem<DTYPE>::kVec;
-  if (col + kVec <= V) {
-    *reinterpret_cast<u32x4_any*>(x + col) = Elem<DTYPE>::pack(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
-      if (col + i < V) x[col + i] = Elem<DTYPE>::down(v[i]);
-  }
-}
-
 // Statistics of a soft-max over part of a row, in powers of two: with rate = log2(e) / tau and a
 // reference c near rate * m, m the maximum so far,
 //   y = rate * x - c (one fused multiply-add),   s = sum 2^y,   w = sum 2^y y.
@@ -218,7 +192,7 @@ __device__ __forceinline__ float row_max(float m, const float (&x)[n]) {
 // lanes of a butterfly end with different last bits.)
 __device__ __forceinline__ void row_stats_move(float& s, float& w, float a, float b) {
 #pragma clang fp contract(off)
-  const float d = fmaxf(a - b, kFarBelow);
+  const float d = a - b;      // finite, both references are
   const float f = __builtin_amdgcn_exp2f(d);
   w = f * (w + s * d);
   s *= f;
