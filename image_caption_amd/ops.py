@@ -397,12 +397,13 @@ def sample_categorical(logits, u, step=0, row_len=None, start_token=-1, eos_toke
 # Forward and gradient are calls of their own, as everywhere in this module (torch supplies memory
 # and streams, not the graph of a backward pass).
 
-def _int32(value, name):
-    """A number the library takes as a 32-bit integer, to which ctypes would cut it without a word."""
-    value = int(value)
-    if not -2 ** 31 <= value < 2 ** 31:
-        raise ValueError("%s %d does not fit 32 bits" % (name, value))
-    return value
+_MAX32 = 2 ** 31 - 1      # sizes and ids go to the library as 32-bit integers, ctypes would cut them without a word
+
+
+def _too_large(**values):
+    for name, value in values.items():
+        if not -_MAX32 - 1 <= value <= _MAX32:
+            raise ValueError("%s %d does not fit 32 bits" % (name, value))
 
 
 def _row_split(t, name):
@@ -478,8 +479,10 @@ def token_log_probs(logits, tokens, top_k=0, pad_token=-1):
     equal logits by the lower id.  Rows whose token is pad_token are left out: zeros, ids of -1."""
     if logits.dim() == 0 or tokens.shape != logits.shape[:-1]:
         raise ValueError("token_log_probs: logits must be [..., V] for tokens [...]")
-    dev, shape, top_k, pad_token = logits.device, tokens.shape, int(top_k), _int32(pad_token, "pad_token")
-    V, N = _int32(logits.shape[-1], "vocabulary"), _int32(tokens.numel(), "number of rows")
+    V, N, dev, shape, top_k = logits.shape[-1], tokens.numel(), logits.device, tokens.shape, int(top_k)
+    pad_token = int(pad_token)
+    if max(V, N, pad_token, ~pad_token) > _MAX32:
+        _too_large(vocabulary=V, rows=N, pad_token=pad_token)
     if not 0 <= top_k <= min(V, _lib.MAX_ALTERNATIVES):
         raise ValueError("token_log_probs: top_k must be in 0 .. min(V, %d)" % _lib.MAX_ALTERNATIVES)
     x, t = _chk(logits, DTYPES, "logits", rows=True), _chk(tokens, i32, "tokens")
@@ -508,8 +511,9 @@ def token_log_probs_grad(logits, tokens, stats, entropy, grad_log_probs=None, gr
     for g in (grad_log_probs, grad_entropy):
         if g is not None and g.shape != tokens.shape:
             raise ValueError("token_log_probs_grad: gradients must have the tokens' shape")
-    V, N = _int32(logits.shape[-1], "vocabulary"), _int32(tokens.numel(), "number of rows")
-    pad_token = _int32(pad_token, "pad_token")
+    V, N, pad_token = logits.shape[-1], tokens.numel(), int(pad_token)
+    if max(V, N, pad_token, ~pad_token) > _MAX32:
+        _too_large(vocabulary=V, rows=N, pad_token=pad_token)
     given, out = out is not None, _grad_out(
         out, logits, "token_log_probs_grad", tokens=tokens, stats=stats, entropy=entropy,
         grad_log_probs=grad_log_probs, grad_entropy=grad_entropy)
@@ -536,8 +540,10 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
     if logits.dim() == 0 or teacher_ids.dim() == 0 or teacher_ids.shape[:-1] != logits.shape[:-1] or \
             teacher_logits.shape != teacher_ids.shape:
         raise ValueError("distill_loss: teacher_logits and teacher_ids must be [..., K] for logits [..., V]")
-    shape, K = logits.shape[:-1], teacher_ids.shape[-1]
-    V, N = _int32(logits.shape[-1], "vocabulary"), _int32(shape.numel(), "number of rows")
+    shape, V, K = logits.shape[:-1], logits.shape[-1], teacher_ids.shape[-1]
+    N = shape.numel()
+    if max(V, N) > _MAX32:
+        _too_large(vocabulary=V, rows=N)
     if V == 0:
         raise ValueError("distill_loss: logits have no columns")
     if not 1 <= K <= _lib.MAX_TEACHER_LOGITS:
@@ -566,8 +572,9 @@ def distill_loss(logits, teacher_logits, teacher_ids, temperature=1.0, grad_loss
 def embedding_scaled(table, ids, scale=1.0, pad_token=-1):
     """scale * table[ids]: table [V,D] (float32, bfloat16 or float16), ids [...] int32 -> [..., D] in
     the table's dtype; zero rows for pad_token and for ids outside the table."""
-    V, D = (_int32(n, "size of the table") for n in table.shape)
-    N, pad_token = _int32(ids.numel(), "number of rows"), _int32(pad_token, "pad_token")
+    (V, D), N, pad_token = table.shape, ids.numel(), int(pad_token)
+    if max(V, D, N, pad_token, ~pad_token) > _MAX32:
+        _too_large(table=max(V, D), rows=N, pad_token=pad_token)
     out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
     tab, i = _chk(table, DTYPES, "table"), _chk(ids, i32, "ids")
     if out.numel():
@@ -581,8 +588,9 @@ def embedding_grad(grad, ids, vocab_size, scale=1.0, pad_token=-1):
     dtype.  Sums run in float32 in an order the ids alone decide: the same inputs, the same bits."""
     if grad.dim() == 0 or grad.shape[:-1] != ids.shape:
         raise ValueError("embedding_grad: grad must be [..., D] for ids [...]")
-    V, D, dev = _int32(vocab_size, "vocab_size"), _int32(grad.shape[-1], "size of a row"), grad.device
-    N, pad_token = _int32(ids.numel(), "number of rows"), _int32(pad_token, "pad_token")
+    V, D, N, dev, pad_token = int(vocab_size), grad.shape[-1], ids.numel(), grad.device, int(pad_token)
+    if max(V, D, N, pad_token, ~pad_token) > _MAX32:
+        _too_large(vocab_size=V, width=D, rows=N, pad_token=pad_token)
     if V < 1:
         raise ValueError("embedding_grad: vocab_size must be positive")
     out = torch.empty(V, D, dtype=grad.dtype, device=dev)
