@@ -155,8 +155,9 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_split_kernel(SortArgs p
 // batch) reads its share again instead.  Every count is an integer and every place follows from
 // the counts, so nothing depends on timing, and no workgroup waits for another.
 // SPLIT: its tokens come from the lists of embed_split_kernel.  Otherwise it reads all of them, 256 x N
-// in all from the caches, which for few tokens is less than a launch: 10240 take 8 us, 131071 took
-// 34 us and take 18 by way of the lists, 6 of them the lists.
+// in all from the caches (2^bits x N for tables of more than 131072 rows), which for few tokens is
+// less than a launch: 10240 take 8 us, 131071 took 34 us and take 18 by way of the lists, 6 of them
+// the lists.
 template <bool SPLIT>
 __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(SortArgs p) {
   __shared__ int s_cnt[kSortWaves][kSortRows];
@@ -468,7 +469,10 @@ struct Workspace {
 };
 
 // Whether the tokens go through lists: from where reading all of them 256 times costs more than a
-// launch, as long as the lists' part for a workgroup fits the lanes that look it up.
+// launch, as long as the lists' part for a workgroup fits the lanes that look it up (2097152 tokens)
+// and the lists' 256 keys are the sorting workgroups (131072 rows of the table).  Past either every
+// workgroup reads all tokens: 131071 tokens x 512 in bf16 take 89 us with 131072 rows and 168 with
+// 131073, rows of 8 into 50000 take 0.68 ms for 2097152 tokens and 2.4 ms for one more.
 bool splits(int N, int V) {
   return N > 24576 && ceil_div(N, kSplitTokens) <= kSplitLists && slots_of(V).bits == 8;
 }

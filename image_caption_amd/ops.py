@@ -397,7 +397,7 @@ def sample_categorical(logits, u, step=0, row_len=None, start_token=-1, eos_toke
 # Forward and gradient are calls of their own, as everywhere in this module (torch supplies memory
 # and streams, not the graph of a backward pass).
 
-_MAX32 = 2 ** 31 - 1      # sizes and ids go to the library as 32-bit integers, ctypes would cut them without a word
+_MAX32 = 2 ** 31 - 1      # sizes and tokens go to the library as 32-bit integers; ctypes cuts them without a word
 
 
 def _too_large(**values):

@@ -92,9 +92,11 @@ class SequenceScorer(object):
     """What the sequence-level trainers need of given sequences next (their policy-gradient steps are
     utils/train_utils.py:397,432,476): __call__((features, sequences)) feeds the policy the
     sequences' tokens and returns, for each token after the first, its log probability and the
-    entropy of the distribution it was drawn from - SequenceScores of [B, T-1] float32, zeros at
-    pad_token; with top_k also the best alternatives [B, T-1, top_k].  `grad` takes gradients of the
-    two back to the logits, [B, T-1, V]."""
+    entropy of the policy's distribution there - SequenceScores of [B, T-1] float32, zeros at
+    pad_token; with top_k also the best alternatives [B, T-1, top_k].  It is the softmax of all the
+    policy's logits: the columns that SequenceSampler masks for its draw take part, and an end token
+    that it forced is scored like any other.  `grad` takes gradients of the two back to the logits,
+    [B, T-1, V]."""
 
     def __init__(self, action_network, pad_token=0, top_k=0):
         self.action_network = action_network
