@@ -425,16 +425,21 @@ def _extent(t):
 
 
 def _apart(a, b):
-    """Whether two tensors of contiguous rows share no byte.  Where their extents meet: every row of
-    either begins a multiple of `step` behind its first, so one's rows may lie between the other's."""
+    """Whether two tensors, contiguous or of contiguous rows, share no byte.  Where their extents meet:
+    every row of either begins a multiple of `step` behind its first, so one's rows may lie between
+    the other's.  A contiguous tensor is one row."""
     if not a.numel() or not b.numel() or a.device != b.device:
         return True
     (a0, a_end), (b0, b_end) = _extent(a), _extent(b)
     if a_end <= b0 or b_end <= a0:
         return True
-    width_a, width_b = ((t.shape[-1] if t.dim() else 1) * t.element_size() for t in (a, b))
-    step = math.gcd(*(st * t.element_size() for t in (a, b) for n, st in zip(t.shape[:-1], t.stride()) if n > 1))
-    return step > 0 and width_b <= (a0 - b0) % step <= step - width_a
+    width, step = [], 0
+    for t in (a, b):
+        size = t.element_size()
+        width.append((t.numel() if t.is_contiguous() else t.shape[-1]) * size)
+        if not t.is_contiguous():
+            step = math.gcd(step, *(st * size for n, st in zip(t.shape[:-1], t.stride()) if n > 1))
+    return step > 0 and width[1] <= (a0 - b0) % step <= step - width[0]
 
 
 def _grad_out(out, like, name, **others):

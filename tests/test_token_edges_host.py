@@ -92,3 +92,18 @@ def test_gradient_over_any_other_operand():
             ops.distill_loss(x, *args, out=out)
     with pytest.raises(ValueError, match="GPU"):
         ops.distill_loss(x, tl, ti, 1.0, pool[32:36], out=out)
+
+
+def test_operands_beside_the_rows_of_a_gradient():
+    """Contiguous operands that lie whole behind one of its rows are no part of it."""
+    from image_caption_amd import ops
+    buf = torch.zeros(4, 40)
+    x, t, out = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32), buf[:, 4:12]
+    st, h, g = buf[1, 12:20].view(4, 2), buf[0, 30:34], buf[2, 12:16]
+    with pytest.raises(ValueError, match="GPU"):
+        ops.token_log_probs_grad(x, t, st, h, g, out=out)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.token_log_probs_grad(buf.view(-1)[92:124].view(4, 8)[:3], t[:3], st[:3], h[:3], g[:3],
+                                 out=buf.as_strided((3, 8), (40, 1), 4))
+    with pytest.raises(ValueError, match="overlaps stats"):
+        ops.token_log_probs_grad(x, t, buf.view(-1)[38:46].view(4, 2), h, g, out=out)
